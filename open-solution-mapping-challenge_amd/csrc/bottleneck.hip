@@ -48,7 +48,7 @@ struct BnkK {
 // s_waitcnt, which also counts the LDS-DMA instructions the compiler cannot see.
 template <int IMM>
 __device__ __forceinline__ void wload(u32x4_t& r, u32x4_t srd, unsigned voff, int soff) {
-    asm volatile("buffer_load_dwordx4 %0, %1, %2, %3 offen offset:%4" : "=v"(r) : "v"(voff), "s"(srd), "s"(soff), "n"(IMM) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2, %3 offen offset:%4" : "=v"(r) : "v"(voff), "s"(srd), "s"(soff), "n"(IMM) : "memory");
 }
 // s_waitcnt vmcnt(N) that the four fragments of a ring slot depend on: the compiler may not touch them before it
 template <int N>

@@ -34,11 +34,16 @@ __device__ __forceinline__ void raw_barrier() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+// Hazard of every vector-memory instruction written as inline asm: an SGPR that a VALU instruction wrote (v_readfirstlane, or the v_readlane of a spilled
+// scalar) must not be read by a vector-memory instruction for five wait states.  The compiler inserts them in front of its own instructions but does not look
+// into asm, so each statement brings its own.  (Without them, a build that schedules v_readfirstlane of the descriptor right in front of the store reads a stale
+// base address: a memory fault in the stem's kernel.)
 // One LDS-DMA wave-instruction: 64 lanes x 16 bytes from buffer offsets `voff` (+ scalar `soff`) to LDS bytes
 // [lds_wave_base, +1024).  Issued through inline asm on purpose: a compiler-visible LDS-DMA makes hipcc put
 // s_waitcnt vmcnt(0) in front of every ds_read of the loop (it cannot disambiguate the ring slots), which
 // serialises the pipeline; hidden from it, the ring is ordered by our own counted vmcnt + s_barrier.
-// M0 (the DMA's LDS base) is compiler-reserved: saved, set and restored inside the one statement.
+// M0 (the DMA's LDS base) is compiler-reserved: saved, set and restored inside the one statement (two s_mov and
+// s_nop 2: the five wait states).
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4_t make_srd(const void* base, unsigned bytes) {
     const unsigned long long b = (unsigned long long)base;
@@ -49,7 +54,7 @@ __device__ __forceinline__ u32x4_t make_srd(const void* base, unsigned bytes) {
 __device__ __forceinline__ void dma16(u32x4_t srd, char* lds_wave_base, unsigned voff, int soff) {
     const unsigned lds_addr = (unsigned)(size_t)(lds_ptr_t)lds_wave_base;
     unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
                  : "s"(lds_addr), "v"(voff), "s"(srd), "s"(soff)
                  : "memory");
@@ -62,7 +67,7 @@ __device__ __forceinline__ void bstore16(u32x4_t srd, unsigned voff, uint4 v) {
     t.x = v.x; t.y = v.y; t.z = v.z; t.w = v.w;
     r.x = __builtin_amdgcn_readfirstlane(srd.x); r.y = __builtin_amdgcn_readfirstlane(srd.y);      // (uniform already; spelled out for the compiler)
     r.z = __builtin_amdgcn_readfirstlane(srd.z); r.w = __builtin_amdgcn_readfirstlane(srd.w);
-    asm volatile("buffer_store_dwordx4 %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(t), "v"(voff), "s"(r) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_store_dwordx4 %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(t), "v"(voff), "s"(r) : "memory");
 }
 
 }  // namespace

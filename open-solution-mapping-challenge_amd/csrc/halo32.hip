@@ -516,7 +516,7 @@ __global__ __launch_bounds__(512) void stem7_halo_kernel(ConvK p, int npatch) {
 // drained the halo requests it cannot see right after they were issued: 74 % of the wave cycles parked, 152 us (SQ_WAIT_ANY, first version).
 // Epilogues: none, or stats_kind 2 (ReLU backward by [sy > 0] + bias-gradient sums); msc_conv_cfg_ok admits nothing else for configuration 59.
 __device__ __forceinline__ void bload16(u32x4_t& r, u32x4_t srd, unsigned voff) {
-    asm volatile("buffer_load_dwordx4 %0, %1, %2, 0 offen" : "=v"(r) : "v"(voff), "s"(srd) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2, 0 offen" : "=v"(r) : "v"(voff), "s"(srd) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_loaded4(u32x4_t (&r)[4]) {
