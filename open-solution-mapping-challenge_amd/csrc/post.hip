@@ -913,7 +913,9 @@ struct CrfHaloR {
 // NORM: the normalisers (sum of the kernel weights over the window clipped to the image) instead of one iteration
 template <int R> struct CrfCols { float gx[2 * R + 1], bx[2 * R + 1]; };      // column factors, computed on the host: kernel arguments = SGPR operands
 
-// ---- round 5: the same kernel on PACKED fp32 math.  The vector peak the roofline quotes (157 TFLOP/s) is the rate of v_pk_fma_f32 -- two
+// ---- The same kernel written on PAIRS of pixels.  It was made for packed fp32 instructions (v_pk_*_f32), which the build now switches off (Makefile: wrong
+// results now and then on this hardware); the pairs are compiled to single operations: the tail with CRF and watershed went from 0.037 to 0.042 ms per image.
+// What follows describes the packed form.  ---- round 5: the same kernel on PACKED fp32 math.  The vector peak the roofline quotes (157 TFLOP/s) is the rate of v_pk_fma_f32 -- two
 // lanes' worth of fp32 FMA per issue slot; scalar-fp32 code tops out at half of it, and the round-4 form (13 VALU + 1 v_exp_f32 per tap and
 // pixel, all unpacked) sat at 0.20 of that peak = 0.40 of what unpacked code can reach.  Here a lane's four vertical pixels are two PAIRS
 // (k, k+1): colour differences, squared distance, exponent argument, the Gaussian factor and the four accumulations are v_pk_* over the
