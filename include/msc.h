@@ -484,6 +484,96 @@ int msc_prep_border(uint8_t* mask_overlayed, const double* second_nearest, doubl
                     void* stream);
 int msc_size_matrix(const int32_t* labels, int32_t* sizes, int32_t* areas, int B, int H, int W, int max_labels, void* stream);
 
+/* ---------------------------------------------------------------- microscaled storage ------------
+ * Tensors held in 8 or 4 bits: activations kept for the backward (msc_mx_pack / _unpack, the weight gradient and the BatchNorm backward that read
+ * them) and the operands of a pointwise convolution = linear layer in serving (msc_mx_linear).  The 16-bit counterparts are msc_pack_cast,
+ * msc_conv_wgrad, msc_bn_bwd_reduce / _apply and the 1x1 form of msc_conv_igemm.  The reference stores and multiplies in float32 only.
+ *
+ * Format.  A tensor is [rows][C] (a row: one pixel of an NHWC tensor, or one token); MSC_MX_BLOCK consecutive channels of a row share a scale.
+ *   codes  : MSC_MX_E4M3 one byte per element; MSC_MX_E2M1 two elements per byte, the even channel in the low nibble.  The last block of a row is
+ *            zero-filled up to MSC_MX_BLOCK, so a row takes nb*32 (nb*16) bytes, nb = ceil(C/32); codes_ld bytes from row to row, a multiple of 16,
+ *            base 16-byte aligned.
+ *   scales : one byte per block, nb bytes per row, scales_ld bytes from row to row.  Byte e stands for 2^(e-127), 255 for NaN.
+ *   value  : code * 2^(e-127).
+ * Packing takes the smallest power of two under which no element passes the largest code (448 / 6) and rounds to the nearest code, ties to even
+ * (an error of at most 2^-4 / 2^-2 of the value, or half the smallest code times the scale).  Elements whose code would stand for a value past the
+ * largest finite one of `dtype` are clamped first (fp16 61440 / 49152, bf16 and f32 1.875 / 1.5 * 2^127).  The scale's byte is at least 10, so that every
+ * value is a normal bf16 number: magnitudes below 2^-127 (2^-119 for E2M1) become zero.  A block that holds an infinity or NaN stands for 32 NaNs.
+ * Everything below runs on `stream`, allocates nothing, synchronises nothing and may be captured; outputs are the same bits from run to run. */
+#define MSC_MX_BLOCK 32
+#define MSC_MX_E4M3 0
+#define MSC_MX_E2M1 1
+int msc_mx_pack(const void* x, int64_t x_ld, int dtype, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int64_t scales_ld, int fmt, int64_t rows,
+                int C, void* stream);
+/* dtype need not be the one that was packed; values past its range become infinities */
+int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, int64_t scales_ld, int fmt, void* out, int64_t out_ld, int dtype,
+                  int64_t rows, int C, void* stream);
+
+/* msc_conv_wgrad with q (the layer's input) held in E4M3:  dw[a][kh][kw][b] (+)= sum_m p[m][a] * q[(y*stride-pad+kh, x*stride-pad+kw)][b], fp32.
+ * The pixel dimension is split over blocks; the partial sums go to `ws` (msc_mx_wgrad_workspace_bytes(d) bytes, may be 0; 16-byte aligned) and are added
+ * in a fixed order.  Any A, B; KH, KW <= 16; p_ld in elements, q_ld / s_ld in bytes.  q's values are exact in every `dtype` they were packed from. */
+typedef struct msc_mx_wgrad_desc {
+    const void* p;
+    const uint8_t* q;
+    const uint8_t* q_scales;
+    float* dw;
+    void* ws;
+    int64_t p_ld, q_ld, s_ld;
+    int32_t dtype;               /* of p */
+    int32_t N, Hp, Wp, A, Hq, Wq, B, KH, KW, stride, pad;
+    int32_t accumulate;          /* 1: dw += ..., 0: dw = ... */
+} msc_mx_wgrad_desc;
+int64_t msc_mx_wgrad_workspace_bytes(const msc_mx_wgrad_desc* d);
+int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream);
+
+/* backward of out = relu?(bn(y) (+ res)), training mode, with y held in E4M3 (msc_bn_bwd_reduce + msc_bn_bwd_apply from a checkpoint):
+ *   dh = dout * mask;  dbeta (+)= sum dh;  dgamma (+)= sum dh*xhat, xhat = (y - mean)*invstd;
+ *   dy = gamma*invstd*(dh - mean(dh) - xhat*mean(dh*xhat));  dres = dh (dres may be NULL; dres_acc: dres += dh)
+ * relu 0: no mask; 2: [scale*y + shift > 0] from the stored y; 3: the byte mask msc_bn_apply wrote (relu_mask, mask_ld bytes per row) -- the
+ * forward's own, which 2 can only approximate.  dy or dres may be dout itself (same ld): each element is read before it is written.
+ * gamma NULL: ones; dgamma / dbeta NULL: not wanted.  ws: msc_mx_bn_bwd_workspace_bytes() bytes, 16-byte aligned. */
+typedef struct msc_mx_bn_bwd_desc {
+    const void* dout;
+    const uint8_t* y;
+    const uint8_t* y_scales;
+    const uint8_t* relu_mask;
+    const float* gamma;
+    const float* mean;
+    const float* invstd;
+    const float* scale;
+    const float* shift;
+    float* dgamma;
+    float* dbeta;
+    void* dy;
+    void* dres;
+    void* ws;
+    int64_t dout_ld, y_ld, s_ld, mask_ld, dy_ld, dres_ld, rows;
+    int32_t dtype, C, relu, accumulate, dres_acc;      /* accumulate: of dgamma / dbeta */
+} msc_mx_bn_bwd_desc;
+int64_t msc_mx_bn_bwd_workspace_bytes(int64_t rows, int C);
+int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream);
+
+/* pointwise convolution / linear layer on E2M1 operands (v_mfma_scale_f32_16x16x128_f8f6f4), fp32 accumulation:
+ *   out[m][n] = act(scale[n] * sum_k x[m][k]*w[n][k] + shift[n] + res[m][n]);   scale / shift / res may be NULL
+ * x: `dtype`, quantised within the call, or already packed (x NULL; x_codes / x_scales).  out and res have `dtype`; res may be out.
+ * x_ld, out_ld, res_ld in elements, the others in bytes.  ws: msc_mx_linear_workspace_bytes(d) bytes (may be 0), 16-byte aligned. */
+typedef struct msc_mx_linear_desc {
+    const void* x;
+    const uint8_t* x_codes;
+    const uint8_t* x_scales;
+    const uint8_t* w;
+    const uint8_t* w_scales;
+    const float* scale;
+    const float* shift;
+    const void* res;
+    void* out;
+    void* ws;
+    int64_t x_ld, xc_ld, xs_ld, w_ld, s_ld, res_ld, out_ld, M;
+    int32_t dtype, K, N, relu;
+} msc_mx_linear_desc;
+int64_t msc_mx_linear_workspace_bytes(const msc_mx_linear_desc* d);
+int msc_mx_linear(const msc_mx_linear_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

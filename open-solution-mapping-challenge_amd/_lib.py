@@ -73,6 +73,28 @@ WGRAD_ORDERED = 1            # msc_wgrad_group_create flags
 FINAL_BWD_WS_ROWS = 1024     # msc_final_bwd ordered_ws rows
 
 
+# microscaled storage (include/msc.h): formats and descriptors
+MX_BLOCK, MX_E4M3, MX_E2M1 = 32, 0, 1
+
+
+class MxWgradDesc(C.Structure):           # == msc_mx_wgrad_desc
+    _fields_ = ([(n, C.c_void_p) for n in ('p', 'q', 'q_scales', 'dw', 'ws')] + [(n, C.c_int64) for n in ('p_ld', 'q_ld', 's_ld')] +
+                [(n, C.c_int32) for n in ('dtype', 'N', 'Hp', 'Wp', 'A', 'Hq', 'Wq', 'B', 'KH', 'KW', 'stride', 'pad', 'accumulate')])
+
+
+class MxBnBwdDesc(C.Structure):           # == msc_mx_bn_bwd_desc
+    _fields_ = ([(n, C.c_void_p) for n in ('dout', 'y', 'y_scales', 'relu_mask', 'gamma', 'mean', 'invstd', 'scale', 'shift', 'dgamma', 'dbeta',
+                                           'dy', 'dres', 'ws')] +
+                [(n, C.c_int64) for n in ('dout_ld', 'y_ld', 's_ld', 'mask_ld', 'dy_ld', 'dres_ld', 'rows')] +
+                [(n, C.c_int32) for n in ('dtype', 'C', 'relu', 'accumulate', 'dres_acc')])
+
+
+class MxLinearDesc(C.Structure):          # == msc_mx_linear_desc
+    _fields_ = ([(n, C.c_void_p) for n in ('x', 'x_codes', 'x_scales', 'w', 'w_scales', 'scale', 'shift', 'res', 'out', 'ws')] +
+                [(n, C.c_int64) for n in ('x_ld', 'xc_ld', 'xs_ld', 'w_ld', 's_ld', 'res_ld', 'out_ld', 'M')] +
+                [(n, C.c_int32) for n in ('dtype', 'K', 'N', 'relu')])
+
+
 class LossCfg(C.Structure):
     _fields_ = [('w0', C.c_float), ('sigma', C.c_float), ('size_c', C.c_float),
                 ('dice_weight', C.c_float), ('ce_weight', C.c_float), ('smooth', C.c_float), ('eps', C.c_float),
@@ -162,6 +184,14 @@ SIGNATURES = {
     'msc_prep_border': (_i, [_vp, _vp, C.c_double, _vp, _i, _i, _vp]),
     'msc_size_matrix': (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     'msc_rle_encode': (_i, [_vp, _i, _i, _i, _i, _vp, _i64, C.POINTER(C.c_int32), C.POINTER(C.c_int64), C.POINTER(_vp), C.POINTER(_vp), _vp]),
+    'msc_mx_pack': (_i, [_vp, _i64, _i, _vp, _i64, _vp, _i64, _i, _i64, _i, _vp]),
+    'msc_mx_unpack': (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i, _i64, _i, _vp]),
+    'msc_mx_wgrad_workspace_bytes': (_i64, [C.POINTER(MxWgradDesc)]),
+    'msc_mx_wgrad': (_i, [C.POINTER(MxWgradDesc), _vp]),
+    'msc_mx_bn_bwd_workspace_bytes': (_i64, [_i64, _i]),
+    'msc_mx_bn_bwd': (_i, [C.POINTER(MxBnBwdDesc), _vp]),
+    'msc_mx_linear_workspace_bytes': (_i64, [C.POINTER(MxLinearDesc)]),
+    'msc_mx_linear': (_i, [C.POINTER(MxLinearDesc), _vp]),
     'msc_dense_crf': (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _f, _f, _f, _f, _f, _i, _vp]),
 }
 

@@ -1,0 +1,378 @@
+// Microscaled storage for gfx950: packing and restoring (msc_mx_pack / msc_mx_unpack) and the BatchNorm backward from an E4M3 checkpoint
+// (msc_mx_bn_bwd).  All three stream their operands once (the BatchNorm twice: its sums come before its result); HBM bounds them.
+#include <stdlib.h>
+
+#include "common.h"
+#include "msc_internal.h"
+#include "mx.h"
+
+namespace {
+
+using namespace mx;
+
+constexpr int THREADS = 256, UNROLL = 4, SPAN = THREADS * UNROLL;
+constexpr int64_t MAX_CHUNKS = 1ll << 30;      // 8-channel chunks of one launch: chunk numbers stay below 2^31; more rows are further launches
+
+// ------------------------------------------------------------------------------------------------ pack
+// A lane takes 8 consecutive channels of a row, a quad of lanes a block: the maximum over the block is two DPP steps, loads (16 bytes a lane for the
+// 16-bit types) and code stores (8 or 4 bytes) are contiguous over the wave.  Four chunks per lane are in flight.  VEC: rows start on 16 bytes
+// and chunks that are whole are loaded as vectors; otherwise element by element (odd widths, channel slices at odd offsets).
+template <typename F, typename T, bool VEC>
+__global__ void pack_kernel(const T* __restrict__ x, long x_ld, uint8_t* __restrict__ codes, long codes_ld, uint8_t* __restrict__ scales, long scales_ld,
+                            unsigned chunks, FastDiv per_row, int C) {
+    const unsigned first = blockIdx.x * (unsigned)SPAN + threadIdx.x;
+    float v[UNROLL][8];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned id = first + u * THREADS;
+        const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
+        const int left = id < chunks ? C - (int)(k * 8) : 0;
+        const T* p = x + (long)row * x_ld + k * 8;
+        if (VEC && left >= 8) load8<T>(p, v[u]);
+        else load8_some<T>(p, left, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned id = first + u * THREADS;
+        const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
+        float q[8];
+        const unsigned e = block_scale<F, T>(v[u], q);
+        if (id >= chunks) continue;              // whole quads: `chunks` is a multiple of four
+        uint8_t* c = codes + (long)row * codes_ld + k * (F::BYTES / 4);
+        if (F::ID == 0) *reinterpret_cast<uint2*>(c) = encode8_e4m3(q);
+        else *reinterpret_cast<unsigned*>(c) = encode8_e2m1(q);
+        if ((k & 3) == 0) scales[(long)row * scales_ld + (k >> 2)] = (uint8_t)e;
+    }
+}
+
+template <typename F, typename T, bool VEC>
+__global__ void unpack_kernel(const uint8_t* __restrict__ codes, long codes_ld, const uint8_t* __restrict__ scales, long scales_ld, T* __restrict__ out,
+                              long out_ld, unsigned chunks, FastDiv per_row, int C) {
+    const unsigned first = blockIdx.x * (unsigned)SPAN + threadIdx.x;
+    uint2 w[UNROLL];
+    unsigned e[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned id = min(first + u * THREADS, chunks - 1);
+        const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
+        const uint8_t* c = codes + (long)row * codes_ld + k * (F::BYTES / 4);
+        if (F::ID == 0) w[u] = *reinterpret_cast<const uint2*>(c);
+        else w[u].x = *reinterpret_cast<const unsigned*>(c);
+        e[u] = scales[(long)row * scales_ld + (k >> 2)];
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned id = first + u * THREADS;
+        if (id >= chunks) continue;
+        const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
+        const float s = scale_value(e[u]);
+        float v[8];
+        if (F::ID == 0) { decode4_e4m3(w[u].x, s, v); decode4_e4m3(w[u].y, s, v + 4); }
+        else decode8_e2m1(w[u].x, s, v);
+        const int left = C - (int)(k * 8);
+        T* p = out + (long)row * out_ld + k * 8;
+        if (VEC && left >= 8) store8<T>(p, v);
+        else store8_some<T>(p, left, v);
+    }
+}
+
+template <typename F, typename T>
+void launch_pack(const void* x, long x_ld, uint8_t* codes, long codes_ld, uint8_t* scales, long scales_ld, unsigned chunks, unsigned per_row, int C, bool vec,
+                 hipStream_t st) {
+    const dim3 grid((chunks + SPAN - 1) / SPAN);
+    auto k = vec ? pack_kernel<F, T, true> : pack_kernel<F, T, false>;
+    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, st, (const T*)x, x_ld, codes, codes_ld, scales, scales_ld, chunks, fast_div(per_row), C);
+}
+template <typename F, typename T>
+void launch_unpack(const uint8_t* codes, long codes_ld, const uint8_t* scales, long scales_ld, void* out, long out_ld, unsigned chunks, unsigned per_row, int C,
+                   bool vec, hipStream_t st) {
+    const dim3 grid((chunks + SPAN - 1) / SPAN);
+    auto k = vec ? unpack_kernel<F, T, true> : unpack_kernel<F, T, false>;
+    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, st, codes, codes_ld, scales, scales_ld, (T*)out, out_ld, chunks, fast_div(per_row), C);
+}
+
+int mx_check(const char* name, const void* x, int64_t x_ld, int dtype, const void* codes, int64_t codes_ld, const void* scales, int64_t scales_ld, int fmt,
+             int64_t rows, int C) {
+    if (fmt != MSC_MX_E4M3 && fmt != MSC_MX_E2M1) return msc_fail(MSC_ERR_ARG, "%s: unknown format %d", name, fmt);
+    if (!msc_dtype_ok(dtype)) return msc_fail(MSC_ERR_ARG, "%s: unknown dtype %d", name, dtype);
+    if (rows < 0 || C <= 0 || C > (1 << 24)) return msc_fail(MSC_ERR_ARG, "%s: bad shape (%lld rows, %d channels)", name, (long long)rows, C);
+    if (rows == 0) return MSC_OK;
+    if (!x || x_ld < C) return msc_fail(MSC_ERR_ARG, "%s: null tensor or row pitch %lld below %d channels", name, (long long)x_ld, C);
+    if ((uintptr_t)x % msc_dtype_size(dtype)) return msc_fail(MSC_ERR_ARG, "%s: tensor not aligned to its elements", name);
+    if (!packed_ok(codes, codes_ld, scales, scales_ld, C, fmt == MSC_MX_E4M3 ? E4M3::BYTES : E2M1::BYTES))
+        return msc_fail(MSC_ERR_ARG, "%s: codes need 16-byte aligned rows of whole blocks, scales one byte per block (row pitches %lld / %lld, %d channels)", name,
+                        (long long)codes_ld, (long long)scales_ld, C);
+    return MSC_OK;
+}
+
+}  // namespace
+
+#define MX_BY_TYPE(F, call)                                              \
+    do {                                                                 \
+        if (dtype == MSC_F32) call<F, float> MX_ARGS;                    \
+        else if (dtype == MSC_BF16) call<F, bf16_t> MX_ARGS;             \
+        else call<F, f16_t> MX_ARGS;                                     \
+    } while (0)
+
+extern "C" int msc_mx_pack(const void* x, int64_t x_ld, int dtype, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int64_t scales_ld, int fmt, int64_t rows,
+                           int C, void* stream) {
+    int rc = mx_check("msc_mx_pack", x, x_ld, dtype, codes, codes_ld, scales, scales_ld, fmt, rows, C);
+    if (rc || rows == 0) return rc;
+    const unsigned per_row = (unsigned)((C + BLOCK - 1) / BLOCK) * 4;
+    const bool vec = vec_ok(x, x_ld, dtype);
+    const int64_t rows_max = MAX_CHUNKS / per_row;
+    for (int64_t r = 0; r < rows; r += rows_max) {
+        const int64_t n = rows - r < rows_max ? rows - r : rows_max;
+        const char* xr = (const char*)x + r * x_ld * msc_dtype_size(dtype);
+#define MX_ARGS (xr, x_ld, codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, (unsigned)(n * per_row), per_row, C, vec, (hipStream_t)stream)
+        if (fmt == MSC_MX_E4M3) MX_BY_TYPE(E4M3, launch_pack);
+        else MX_BY_TYPE(E2M1, launch_pack);
+#undef MX_ARGS
+    }
+    return msc_check_launch("msc_mx_pack");
+}
+
+extern "C" int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, int64_t scales_ld, int fmt, void* out, int64_t out_ld, int dtype,
+                             int64_t rows, int C, void* stream) {
+    int rc = mx_check("msc_mx_unpack", out, out_ld, dtype, codes, codes_ld, scales, scales_ld, fmt, rows, C);
+    if (rc || rows == 0) return rc;
+    const unsigned per_row = (unsigned)((C + BLOCK - 1) / BLOCK) * 4;
+    const bool vec = vec_ok(out, out_ld, dtype);
+    const int64_t rows_max = MAX_CHUNKS / per_row;
+    for (int64_t r = 0; r < rows; r += rows_max) {
+        const int64_t n = rows - r < rows_max ? rows - r : rows_max;
+        char* o = (char*)out + r * out_ld * msc_dtype_size(dtype);
+#define MX_ARGS (codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, o, out_ld, (unsigned)(n * per_row), per_row, C, vec, (hipStream_t)stream)
+        if (fmt == MSC_MX_E4M3) MX_BY_TYPE(E4M3, launch_unpack);
+        else MX_BY_TYPE(E2M1, launch_unpack);
+#undef MX_ARGS
+    }
+    return msc_check_launch("msc_mx_unpack");
+}
+
+// ------------------------------------------------------------------------------------------------ BatchNorm backward
+// Three launches.  reduce: a block takes a strip of rows and up to 256 channels (a lane 8 of them), sums dh and dh*(y - mean) in fp32 over its rows, in
+// double over its row groups, and leaves one partial per channel.  finish: adds the strips' partials in order (double), writes dgamma / dbeta and the
+// coefficients of dy = a*dh + c2*(y - mean) + c1.  apply: streams again.  Centring y by the batch mean before the products keeps the sum from losing what
+// a large mean would cancel.
+namespace {
+
+constexpr int BN_COLS = 32;                    // 8-channel chunks of a block's column range at most
+
+struct BnArgs {
+    const void* dout; const uint8_t* y; const uint8_t* y_scales; const uint8_t* mask;
+    const float* mean; const float* invstd; const float* gamma; const float* scale; const float* shift;
+    float* dgamma; float* dbeta; void* dy; void* dres;
+    double2* part; float4* coef;
+    long dout_ld, y_ld, s_ld, mask_ld, dy_ld, dres_ld, rows, strip;
+    int C, strips, cols_log2, accumulate, dres_acc;
+};
+
+// the 8 masked gradients and centred inputs of one chunk
+template <typename T, int RELU, bool VEC>
+__device__ __forceinline__ void bn_chunk(const BnArgs& a, long row, int c0, int left, const float* mean, const float* sc, const float* sh, float* dh, float* t) {
+    const T* d = (const T*)a.dout + row * a.dout_ld + c0;
+    if (VEC && left >= 8) load8<T>(d, dh);
+    else load8_some<T>(d, left, dh);
+    const uint2 w = *reinterpret_cast<const uint2*>(a.y + row * a.y_ld + c0);
+    const float s = scale_value(a.y_scales[row * a.s_ld + (c0 >> 5)]);
+    float y[8];
+    decode4_e4m3(w.x, s, y);
+    decode4_e4m3(w.y, s, y + 4);
+    unsigned bits = 0xff;
+    if (RELU == 3) {
+        const uint8_t* m = a.mask + row * a.mask_ld;
+        if (sizeof(T) == 2) bits = m[c0 >> 3];
+        else bits = (m[c0 >> 2] & 15u) | (left > 4 ? (unsigned)m[(c0 >> 2) + 1] << 4 : 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (RELU == 2) dh[i] = fmaf(sc[i], y[i], sh[i]) > 0.f ? dh[i] : 0.f;
+        if (RELU == 3) dh[i] = (bits >> i) & 1 ? dh[i] : 0.f;
+        t[i] = y[i] - mean[i];
+    }
+}
+
+template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
+    __shared__ float2 red[THREADS][9];         // 8 channels per thread, one column of padding
+    const int cols = 1 << a.cols_log2;
+    const int col = threadIdx.x & (cols - 1), rg = threadIdx.x >> a.cols_log2, groups = THREADS >> a.cols_log2;
+    const int c0 = (blockIdx.y * cols + col) * 8, left = a.C - c0;
+    float s1[8], s2[8], mean[8], sc[8], sh[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s1[i] = s2[i] = 0.f;
+        mean[i] = i < left ? a.mean[c0 + i] : 0.f;
+        sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
+        sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
+    }
+    const long r1 = min(a.rows, (long)(blockIdx.x + 1) * a.strip);
+    if (left > 0)
+        for (long r = (long)blockIdx.x * a.strip + rg; r < r1; r += groups) {
+            float dh[8], t[8];
+            bn_chunk<T, RELU, VEC>(a, r, c0, left, mean, sc, sh, dh, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { s1[i] += dh[i]; s2[i] = fmaf(dh[i], t[i], s2[i]); }
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[threadIdx.x][i] = make_float2(s1[i], s2[i]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols * 8; c += THREADS) {
+        const int ch = blockIdx.y * cols * 8 + c;
+        double2 s = make_double2(0.0, 0.0);
+        for (int g = 0; g < groups; ++g) {
+            const float2 v = red[(g << a.cols_log2) + (c >> 3)][c & 7];
+            s.x += v.x; s.y += v.y;
+        }
+        if (ch < a.C) a.part[(long)blockIdx.x * a.C + ch] = s;
+    }
+}
+
+// FIN channels x THREADS / FIN slices of the strips per block
+constexpr int FIN = 4;
+__global__ __launch_bounds__(256) void bn_finish_kernel(BnArgs a) {
+    __shared__ double2 red[THREADS];
+    constexpr int SLICES = THREADS / FIN;
+    const int c = threadIdx.x % FIN, k = threadIdx.x / FIN, ch = blockIdx.x * FIN + c;
+    double2 s = make_double2(0.0, 0.0);
+    if (ch < a.C) {
+        int i = k;
+        for (; i + 3 * SLICES < a.strips; i += 4 * SLICES) {
+            double2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = a.part[(long)(i + u * SLICES) * a.C + ch];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { s.x += v[u].x; s.y += v[u].y; }
+        }
+        for (; i < a.strips; i += SLICES) {
+            const double2 v = a.part[(long)i * a.C + ch];
+            s.x += v.x; s.y += v.y;
+        }
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int h = SLICES / 2; h; h >>= 1) {
+        if (k < h) {
+            const double2 v = red[threadIdx.x + h * FIN];
+            s.x += v.x; s.y += v.y;
+            red[threadIdx.x] = s;
+        }
+        __syncthreads();
+    }
+    if (k || ch >= a.C) return;
+    const double inv = a.invstd[ch], n = (double)a.rows;
+    const double db = s.x, dg = s.y * inv, ga = (a.gamma ? (double)a.gamma[ch] : 1.0) * inv;
+    a.coef[ch] = make_float4((float)ga, (float)(-ga * db / n), (float)(-ga * inv * dg / n), a.mean[ch]);
+    if (a.dgamma) a.dgamma[ch] = (a.accumulate ? a.dgamma[ch] : 0.f) + (float)dg;
+    if (a.dbeta) a.dbeta[ch] = (a.accumulate ? a.dbeta[ch] : 0.f) + (float)db;
+}
+
+template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
+    const int cols = 1 << a.cols_log2;
+    const int col = threadIdx.x & (cols - 1), rg = threadIdx.x >> a.cols_log2, groups = THREADS >> a.cols_log2;
+    const int c0 = (blockIdx.y * cols + col) * 8, left = a.C - c0;
+    if (left <= 0) return;
+    float ga[8], c1[8], c2[8], mean[8], sc[8], sh[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 f = i < left ? a.coef[c0 + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        ga[i] = f.x; c1[i] = f.y; c2[i] = f.z; mean[i] = f.w;
+        sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
+        sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
+    }
+    const long r1 = min(a.rows, (long)(blockIdx.x + 1) * a.strip);
+    for (long r = (long)blockIdx.x * a.strip + rg; r < r1; r += groups) {
+        float dh[8], t[8];
+        bn_chunk<T, RELU, VEC>(a, r, c0, left, mean, sc, sh, dh, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = fmaf(ga[i], dh[i], fmaf(c2[i], t[i], c1[i]));
+        T* o = (T*)a.dy + r * a.dy_ld + c0;
+        if (a.dres) {
+            T* g = (T*)a.dres + r * a.dres_ld + c0;
+            if (a.dres_acc) {
+                float old[8];
+                if (VEC && left >= 8) load8<T>(g, old);
+                else load8_some<T>(g, left, old);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dh[i] += old[i];
+            }
+            if (VEC && left >= 8) store8<T>(g, dh);
+            else store8_some<T>(g, left, dh);
+        }
+        if (VEC && left >= 8) store8<T>(o, t);
+        else store8_some<T>(o, left, t);
+    }
+}
+
+struct BnPlan { int cols_log2, ctiles, strips; long strip; };
+BnPlan bn_plan(int64_t rows, int C) {
+    BnPlan p;
+    const int chunks = (C + 7) / 8;
+    p.cols_log2 = 0;
+    while ((1 << p.cols_log2) < chunks && (1 << p.cols_log2) < BN_COLS) ++p.cols_log2;
+    p.ctiles = (chunks + (1 << p.cols_log2) - 1) >> p.cols_log2;
+    const int groups = THREADS >> p.cols_log2;
+    // about 1024 blocks in all, at least four rows per thread
+    long strips = 1024 / p.ctiles, most = (rows + groups * 4 - 1) / (groups * 4);
+    if (strips > most) strips = most;
+    if (strips < 1) strips = 1;
+    p.strip = (rows + strips - 1) / strips;
+    p.strip = (p.strip + groups - 1) / groups * groups;
+    p.strips = (int)((rows + p.strip - 1) / p.strip);
+    return p;
+}
+
+template <typename T, int RELU> void bn_launch(const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
+    const dim3 grid(p.strips, p.ctiles);
+    hipLaunchKernelGGL((vec ? bn_reduce_kernel<T, RELU, true> : bn_reduce_kernel<T, RELU, false>), grid, dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL(bn_finish_kernel, dim3((a.C + FIN - 1) / FIN), dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((vec ? bn_apply_kernel<T, RELU, true> : bn_apply_kernel<T, RELU, false>), grid, dim3(THREADS), 0, st, a);
+}
+template <typename T> void bn_by_relu(int relu, const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
+    if (relu == 0) bn_launch<T, 0>(a, p, vec, st);
+    else if (relu == 2) bn_launch<T, 2>(a, p, vec, st);
+    else bn_launch<T, 3>(a, p, vec, st);
+}
+
+}  // namespace
+
+extern "C" int64_t msc_mx_bn_bwd_workspace_bytes(int64_t rows, int C) {
+    if (rows <= 0 || C <= 0 || C > (1 << 24)) return 0;
+    return (int64_t)C * 16 * (1 + bn_plan(rows, C).strips);
+}
+
+extern "C" int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream) {
+    if (!d) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: null descriptor");
+    if (!msc_dtype_ok(d->dtype)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: unknown dtype %d", d->dtype);
+    if (d->rows <= 0 || d->C <= 0 || d->C > (1 << 24))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: bad shape (%lld rows, %d channels)", (long long)d->rows, d->C);
+    if (!d->dout || !d->dy || !d->mean || !d->invstd || !d->ws) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: null pointer");
+    if (d->relu != 0 && d->relu != 2 && d->relu != 3) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: relu is 0, 2 or 3, got %d", d->relu);
+    if (d->relu == 2 && (!d->scale || !d->shift)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: relu 2 needs scale and shift");
+    const int per = msc_dtype_vec(d->dtype);
+    if (d->relu == 3 && (!d->relu_mask || d->mask_ld < (d->C + per - 1) / per))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: relu 3 needs the byte mask, %d bytes per row", (d->C + per - 1) / per);
+    if (d->dout_ld < d->C || d->dy_ld < d->C || (d->dres && d->dres_ld < d->C)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: row pitch below %d channels", d->C);
+    if (!packed_ok(d->y, d->y_ld, d->y_scales, d->s_ld, d->C, E4M3::BYTES))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: y needs 16-byte aligned rows of whole E4M3 blocks and one scale byte per block");
+    if ((uintptr_t)d->ws & 15) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: workspace not 16-byte aligned");
+    const int es = msc_dtype_size(d->dtype);
+    if ((uintptr_t)d->dout % es || (uintptr_t)d->dy % es || (uintptr_t)d->dres % es) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: tensor not aligned to its elements");
+    if ((d->dy == d->dout && d->dy_ld != d->dout_ld) || (d->dres == d->dout && d->dres_ld != d->dout_ld) || d->dres == d->dy)
+        return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: dy and dres are different buffers; either may be dout, with its row pitch");
+    const BnPlan p = bn_plan(d->rows, d->C);
+    if (p.ctiles > 65535) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_bn_bwd: too many channels");
+    BnArgs a;
+    a.dout = d->dout; a.y = d->y; a.y_scales = d->y_scales; a.mask = d->relu_mask;
+    a.mean = d->mean; a.invstd = d->invstd; a.gamma = d->gamma; a.scale = d->scale; a.shift = d->shift;
+    a.dgamma = d->dgamma; a.dbeta = d->dbeta; a.dy = d->dy; a.dres = d->dres;
+    a.coef = (float4*)d->ws; a.part = (double2*)((char*)d->ws + (int64_t)d->C * 16);
+    a.dout_ld = d->dout_ld; a.y_ld = d->y_ld; a.s_ld = d->s_ld; a.mask_ld = d->mask_ld; a.dy_ld = d->dy_ld; a.dres_ld = d->dres_ld;
+    a.rows = d->rows; a.strip = p.strip; a.C = d->C; a.strips = p.strips; a.cols_log2 = p.cols_log2; a.accumulate = d->accumulate; a.dres_acc = d->dres_acc;
+    const bool vec = vec_ok(d->dout, d->dout_ld, d->dtype) && vec_ok(d->dy, d->dy_ld, d->dtype) && (!d->dres || vec_ok(d->dres, d->dres_ld, d->dtype));
+    hipStream_t st = (hipStream_t)stream;
+    if (d->dtype == MSC_F32) bn_by_relu<float>(d->relu, a, p, vec, st);
+    else if (d->dtype == MSC_BF16) bn_by_relu<bf16_t>(d->relu, a, p, vec, st);
+    else bn_by_relu<f16_t>(d->relu, a, p, vec, st);
+    return msc_check_launch("msc_mx_bn_bwd");
+}

@@ -1,0 +1,276 @@
+"""Microscaled storage on the device: tensors in 8 or 4 bits with one power-of-two scale per 32 channels (include/msc.h, msc_mx_*).
+
+The reference trains and serves in float32 and has no counterpart; these stand beside the engine's 16-bit operators:
+
+  pack / unpack        a tensor to E4M3 (one byte per element) or E2M1 (half a byte) and back; beside msc_pack_cast
+  conv_weight_grad     weight gradient of a convolution / linear layer from the E4M3 checkpoint of its input; beside msc_conv_wgrad
+  batchnorm_backward   BatchNorm (+ ReLU, + residual join) backward from the E4M3 checkpoint of its input; beside msc_bn_bwd_reduce / _apply
+  linear               a pointwise convolution / linear layer on E2M1 operands, for serving; beside the 1x1 form of msc_conv_igemm
+
+Tensors are [..., C], a row of channels per pixel or token: NHWC activations, a channel slice of one, or [rows, C].  float32, bfloat16 and float16.
+Calls run on the current stream of the tensors' device, take their scratch from torch's allocator, never synchronise and may be captured into a
+hipGraph; results are the same bits from run to run.  Nothing is recorded by autograd.
+
+A training step that keeps its activations in 8 bits calls pack behind each layer's forward and conv_weight_grad / batchnorm_backward in its backward:
+UNetResNet(activation_checkpoint='e4m3') does so.
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+FORMATS = {'e4m3': (_lib.MX_E4M3, 32), 'e2m1': (_lib.MX_E2M1, 16)}       # name -> (id, bytes of a block's codes)
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+class MxTensor:
+    """A packed tensor of shape [..., channels]: codes uint8 [..., blocks * 32 (E4M3) or 16 (E2M1)], scales uint8 [..., blocks], blocks = ceil(channels / 32).
+    Rows of codes start on 16 bytes; both may be slices of wider buffers."""
+    __slots__ = ('codes', 'scales', 'channels', 'fmt')
+
+    def __init__(self, codes, scales, channels, fmt='e4m3'):
+        if fmt not in FORMATS:
+            raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
+        nb = (channels + 31) // 32
+        if channels <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError('a packed tensor has at least one channel, and uint8 codes and scales')
+        if codes.shape[-1] != nb * FORMATS[fmt][1] or scales.shape[-1] != nb or codes.shape[:-1] != scales.shape[:-1]:
+            raise ValueError('%d channels in %s take %d code bytes and %d scales per row, got codes %s and scales %s'
+                             % (channels, fmt, nb * FORMATS[fmt][1], nb, tuple(codes.shape), tuple(scales.shape)))
+        if codes.device != scales.device:
+            raise ValueError('codes and scales are on different devices')
+        self.codes, self.scales, self.channels, self.fmt = codes, scales, channels, fmt
+
+    @property
+    def shape(self):
+        return tuple(self.codes.shape[:-1]) + (self.channels,)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def _rows(t, what):
+    """(rows, elements from row to row) of a tensor [..., C] whose rows are equally far apart"""
+    if not t.is_cuda:
+        raise _lib.MscError('%s: needs a CUDA/ROCm tensor; there is no CPU path in the product' % what)
+    if t.dim() < 2:
+        raise ValueError('%s: expected [..., channels], got shape %s' % (what, tuple(t.shape)))
+    if t.is_contiguous():
+        return t.numel() // t.shape[-1] if t.shape[-1] else 0, t.shape[-1]
+    shape, stride = t.shape, t.stride()
+    if shape[-1] > 1 and stride[-1] != 1:
+        raise ValueError('%s: channels have to be next to each other (strides %s)' % (what, tuple(stride)))
+    pitch, rows = None, 1
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n != 1:
+            if pitch is None:
+                pitch = s
+            elif s != pitch * rows:
+                raise ValueError('%s: expected an NHWC tensor or a channel slice of one (shape %s, strides %s)' % (what, tuple(shape), tuple(stride)))
+        rows *= n
+    return rows, max(shape[-1], 1) if pitch is None or rows == 0 else pitch
+
+
+def _dtype(t, what):
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError('%s: float32, bfloat16 or float16, got %s' % (what, t.dtype)) from None
+
+
+def _same_device(what, dev, *ts):
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError('%s: tensors on %s and %s' % (what, dev, t.device))
+
+
+def _vector(t, n, dev, what):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise ValueError('%s: expected %d contiguous float32 values on %s' % (what, n, dev))
+    return t.data_ptr()
+
+
+def _out(out, shape, dtype, dev, what):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev:
+        raise ValueError('%s: out has to be %s %s on %s' % (what, tuple(shape), dtype, dev))
+    return out
+
+
+def _run(name, dev, *args):
+    """one C call on `dev`'s current stream, with `dev` current"""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    # the handle alone: the Stream object that torch.cuda.current_stream() makes costs as much as a launch's own host time
+    _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+def _workspace(name, nbytes, dev):
+    if nbytes < 0:
+        _lib.check(-1, name)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def empty(shape, fmt='e4m3', device='cuda'):
+    """an uninitialised MxTensor of `shape` [..., channels]"""
+    nb = (shape[-1] + 31) // 32
+    lead = tuple(shape[:-1])
+    return MxTensor(torch.empty(lead + (nb * FORMATS[fmt][1],), dtype=torch.uint8, device=device),
+                    torch.empty(lead + (nb,), dtype=torch.uint8, device=device), shape[-1], fmt)
+
+
+def pack(x, fmt='e4m3', out=None):
+    """x [..., C] in blocks of 32 channels: the smallest power-of-two scale under which nothing passes the largest code, then the nearest code (ties to
+    even).  A block that holds an infinity or NaN stands for 32 NaNs.  Returns an MxTensor (`out`, if given)."""
+    if fmt not in FORMATS:
+        raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
+    rows, ld = _rows(x, 'pack')
+    dt = _dtype(x, 'pack')
+    if out is None:
+        out = empty(x.shape, fmt, x.device)
+    elif out.shape != tuple(x.shape) or out.fmt != fmt:
+        raise ValueError('pack: out holds %s in %s, not %s in %s' % (out.shape, out.fmt, tuple(x.shape), fmt))
+    _same_device('pack', x.device, out.codes)
+    _run('msc_mx_pack', x.device, x.data_ptr(), ld, dt, out.codes.data_ptr(), _rows(out.codes, 'pack')[1], out.scales.data_ptr(),
+         _rows(out.scales, 'pack')[1], FORMATS[fmt][0], rows, x.shape[-1])
+    return out
+
+
+def unpack(t, dtype=torch.bfloat16, out=None):
+    """the values an MxTensor stands for, in `dtype` (any of the three; the one that was packed holds every value exactly)"""
+    out = _out(out, t.shape, dtype if out is None else out.dtype, t.device, 'unpack')
+    rows, ld = _rows(out, 'unpack')
+    _run('msc_mx_unpack', t.device, t.codes.data_ptr(), _rows(t.codes, 'unpack')[1], t.scales.data_ptr(), _rows(t.scales, 'unpack')[1], FORMATS[t.fmt][0],
+         out.data_ptr(), ld, _dtype(out, 'unpack'), rows, t.channels)
+    return out
+
+
+def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=False):
+    """float32 [A, KH, KW, B]: the weight gradient of a convolution whose output gradient is dy [N, H, W, A] and whose input [N, Hi, Wi, B] was kept as the E4M3
+    MxTensor `saved`.  kernel: a size or (KH, KW).  A linear layer: kernel 1, dy [..., A] and saved [..., B] with the same leading shape.
+    accumulate: added to `out` (which then has to be given) instead of written over it."""
+    if saved.fmt != 'e4m3':
+        raise ValueError('conv_weight_grad: the checkpoint has to be in e4m3, got %s' % saved.fmt)
+    if accumulate and out is None:
+        raise ValueError('conv_weight_grad: accumulate needs out')
+    kh, kw = (kernel, kernel) if isinstance(kernel, int) else kernel
+    rows, p_ld = _rows(dy, 'conv_weight_grad')
+    _, q_ld = _rows(saved.codes, 'conv_weight_grad')
+    _, s_ld = _rows(saved.scales, 'conv_weight_grad')
+    a, b = dy.shape[-1], saved.channels
+    d = _lib.MxWgradDesc()
+    if kh == 1 and kw == 1 and stride == 1 and pad == 0:
+        if tuple(dy.shape[:-1]) != saved.shape[:-1]:
+            raise ValueError('conv_weight_grad: dy %s and input %s differ in their rows' % (tuple(dy.shape), saved.shape))
+        d.N, d.Hp, d.Wp, d.Hq, d.Wq = rows, 1, 1, 1, 1
+    else:
+        if dy.dim() != 4 or len(saved.shape) != 4 or dy.shape[0] != saved.shape[0]:
+            raise ValueError('conv_weight_grad: expected NHWC dy and input, got %s and %s' % (tuple(dy.shape), saved.shape))
+        (d.N, d.Hp, d.Wp), (d.Hq, d.Wq) = dy.shape[:3], saved.shape[1:3]
+        want = tuple((i + 2 * pad - k) // stride + 1 if stride > 0 else 0 for i, k in ((d.Hq, kh), (d.Wq, kw)))
+        if (d.Hp, d.Wp) != want:
+            raise ValueError('conv_weight_grad: an input of %dx%d gives an output of %dx%d, dy is %dx%d' % (d.Hq, d.Wq, want[0], want[1], d.Hp, d.Wp))
+    dev = dy.device
+    out = _out(out, (a, kh, kw, b), torch.float32, dev, 'conv_weight_grad')
+    if not out.is_contiguous():
+        raise ValueError('conv_weight_grad: out has to be contiguous')
+    _same_device('conv_weight_grad', dev, saved.codes)
+    d.p, d.q, d.q_scales, d.dw = dy.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), out.data_ptr()
+    d.p_ld, d.q_ld, d.s_ld, d.dtype = p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad')
+    d.A, d.B, d.KH, d.KW, d.stride, d.pad, d.accumulate = a, b, kh, kw, stride, pad, int(accumulate)
+    ref = C.byref(d)
+    ws = _workspace('msc_mx_wgrad_workspace_bytes', _lib.load().msc_mx_wgrad_workspace_bytes(ref), dev)
+    d.ws = None if ws is None else ws.data_ptr()
+    _run('msc_mx_wgrad', dev, ref)
+    return out
+
+
+def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=None, shift=None, residual=False, dy=None):
+    """Backward of out = relu?(batchnorm(y) (+ res)) in training mode, with y [..., C] kept as the E4M3 MxTensor `saved` and mean / invstd the forward's
+    batch statistics: (dy, dgamma, dbeta) or, with residual, (dy, dgamma, dbeta, dres).
+    The ReLU: relu_mask, the byte mask msc_bn_apply writes ([..., ceil(C / 8)], for float32 ceil(C / 4)); or scale and shift, the forward's coefficients, from
+    which the mask is recomputed on the stored y; or neither: no ReLU.  gamma may be None (ones).  dy may be dout (in place)."""
+    if saved.fmt != 'e4m3':
+        raise ValueError('batchnorm_backward: the checkpoint has to be in e4m3, got %s' % saved.fmt)
+    if tuple(dout.shape) != saved.shape:
+        raise ValueError('batchnorm_backward: dout %s and input %s differ' % (tuple(dout.shape), saved.shape))
+    if (scale is None) != (shift is None) or (scale is not None and relu_mask is not None):
+        raise ValueError('batchnorm_backward: the ReLU takes relu_mask, or scale and shift, or neither')
+    dev, c = dout.device, saved.channels
+    d = _lib.MxBnBwdDesc()
+    d.rows, d.dout_ld = _rows(dout, 'batchnorm_backward')
+    _, d.y_ld = _rows(saved.codes, 'batchnorm_backward')
+    _, d.s_ld = _rows(saved.scales, 'batchnorm_backward')
+    _same_device('batchnorm_backward', dev, saved.codes, relu_mask)
+    d.dtype, d.C = _dtype(dout, 'batchnorm_backward'), c
+    if relu_mask is not None:
+        per = 4 if dout.dtype == torch.float32 else 8
+        if relu_mask.dtype != torch.uint8 or tuple(relu_mask.shape) != tuple(dout.shape[:-1]) + ((c + per - 1) // per,):
+            raise ValueError('batchnorm_backward: the mask has one byte for %d channels of a row, got %s %s' % (per, tuple(relu_mask.shape), relu_mask.dtype))
+        d.relu, d.relu_mask, d.mask_ld = 3, relu_mask.data_ptr(), _rows(relu_mask, 'batchnorm_backward')[1]
+    elif scale is not None:
+        d.relu, d.scale, d.shift = 2, _vector(scale, c, dev, 'batchnorm_backward: scale'), _vector(shift, c, dev, 'batchnorm_backward: shift')
+    d.gamma = _vector(gamma, c, dev, 'batchnorm_backward: gamma')
+    d.mean, d.invstd = _vector(mean, c, dev, 'batchnorm_backward: mean'), _vector(invstd, c, dev, 'batchnorm_backward: invstd')
+    dy = _out(dy, dout.shape, dout.dtype, dev, 'batchnorm_backward')
+    d.dy_ld = _rows(dy, 'batchnorm_backward')[1]
+    dgamma, dbeta = torch.empty((2, c), dtype=torch.float32, device=dev)
+    d.dout, d.y, d.y_scales, d.dy = dout.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), dy.data_ptr()
+    d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
+    dres = None
+    if residual:
+        dres = torch.empty(dout.shape, dtype=dout.dtype, device=dev)
+        d.dres, d.dres_ld = dres.data_ptr(), c
+    ws = _workspace('msc_mx_bn_bwd_workspace_bytes', _lib.load().msc_mx_bn_bwd_workspace_bytes(d.rows, c), dev)
+    d.ws = None if ws is None else ws.data_ptr()
+    _run('msc_mx_bn_bwd', dev, C.byref(d))
+    return (dy, dgamma, dbeta, dres) if residual else (dy, dgamma, dbeta)
+
+
+def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=None):
+    """act(scale * (x @ w.T) + shift + res) [..., N]: x [..., K] a tensor (quantised to E2M1 within the call) or an E2M1 MxTensor (dtype: the result's,
+    bfloat16 if not given), w the E2M1 MxTensor of a weight [N, K]; scale / shift float32 [N] (a folded BatchNorm, a bias), res [..., N] in the result's
+    dtype.  out may be res."""
+    packed = isinstance(x, MxTensor)
+    if w.fmt != 'e2m1' or (packed and x.fmt != 'e2m1'):
+        raise ValueError('linear: the operands have to be in e2m1')
+    if len(w.shape) != 2 or w.channels != x.shape[-1]:
+        raise ValueError('linear: x %s and w %s do not go together' % (tuple(x.shape), w.shape))
+    dev, (n, k) = x.device, w.shape
+    if dtype is None:
+        dtype = out.dtype if out is not None else x.dtype if not packed else res.dtype if res is not None else torch.bfloat16
+    if not packed and x.dtype != dtype:
+        raise ValueError('linear: the result has the type of x')
+    out = _out(out, tuple(x.shape[:-1]) + (n,), dtype, dev, 'linear')
+    _same_device('linear', dev, w.codes)
+    d = _lib.MxLinearDesc()
+    if packed:
+        d.M, d.xc_ld = _rows(x.codes, 'linear')
+        d.x_codes, d.x_scales, d.xs_ld = x.codes.data_ptr(), x.scales.data_ptr(), _rows(x.scales, 'linear')[1]
+    else:
+        d.M, d.x_ld = _rows(x, 'linear')
+        d.x = x.data_ptr()
+    d.w, d.w_scales, d.w_ld, d.s_ld = w.codes.data_ptr(), w.scales.data_ptr(), _rows(w.codes, 'linear')[1], _rows(w.scales, 'linear')[1]
+    d.scale, d.shift = _vector(scale, n, dev, 'linear: scale'), _vector(shift, n, dev, 'linear: shift')
+    if res is not None:
+        _out(res, out.shape, dtype, dev, 'linear: res')
+        d.res, d.res_ld = res.data_ptr(), _rows(res, 'linear')[1]
+    d.out, d.out_ld = out.data_ptr(), _rows(out, 'linear')[1]
+    d.dtype, d.K, d.N, d.relu = _dtype(out, 'linear'), k, n, int(relu)
+    if d.M == 0:
+        return out
+    ref = C.byref(d)
+    ws = _workspace('msc_mx_linear_workspace_bytes', _lib.load().msc_mx_linear_workspace_bytes(ref), dev)
+    d.ws = None if ws is None else ws.data_ptr()
+    _run('msc_mx_linear', dev, ref)
+    return out
