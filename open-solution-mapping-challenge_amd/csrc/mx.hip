@@ -151,12 +151,15 @@ extern "C" int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8
 }
 
 // ------------------------------------------------------------------------------------------------ BatchNorm backward
-// Three launches.  reduce: a block takes a strip of rows and up to 256 channels (a lane 8 of them), sums dh and dh*(y - mean) in fp32 over its rows, in
-// double over its row groups, and leaves one partial per channel.  finish: adds the strips' partials in order (double), writes dgamma / dbeta and the
+// Three launches.  reduce: a block takes every n-th few rows and up to 256 channels (a lane 8 of them), sums dh and dh*(y - mean) in fp32 over its rows, in
+// double over its row groups, and leaves one partial per channel.  finish: adds the blocks' partials in order (double), writes dgamma / dbeta and the
 // coefficients of dy = a*dh + c2*(y - mean) + c1.  apply: streams again.  Centring y by the batch mean before the products keeps the sum from losing what
 // a large mean would cancel.
 namespace {
 
+// Rows in flight per thread, and blocks.  131072 x 256 bf16 join: reduce 34.6 us with one row, 31-32 with two or four (3.4 TB/s: a plain read-only sum of 1 GB reaches 4.0
+// on the card), 36 with half the blocks; apply 51 with one, 42 with two (the second reading of dout and y is from the last-level cache), 48 with 8192 blocks.
+constexpr int BN_ROWS = 4, BN_APPLY_ROWS = 2, BN_BLOCKS = 1024, BN_APPLY_BLOCKS = 2048;
 constexpr int BN_COLS = 32;                    // 8-channel chunks of a block's column range at most
 
 struct BnArgs {
@@ -164,31 +167,35 @@ struct BnArgs {
     const float* mean; const float* invstd; const float* gamma; const float* scale; const float* shift;
     float* dgamma; float* dbeta; void* dy; void* dres;
     double2* part; float4* coef;
-    long dout_ld, y_ld, s_ld, mask_ld, dy_ld, dres_ld, rows, strip;
+    long dout_ld, y_ld, s_ld, mask_ld, dy_ld, dres_ld, rows;
     int C, strips, cols_log2, accumulate, dres_acc;
 };
 
-// the 8 masked gradients and centred inputs of one chunk
-template <typename T, int RELU, bool VEC>
-__device__ __forceinline__ void bn_chunk(const BnArgs& a, long row, int c0, int left, const float* mean, const float* sc, const float* sh, float* dh, float* t) {
+// what one chunk (8 channels of a row) reads, and its masked gradients and centred inputs: apart, so that several rows' loads are in flight
+struct BnRaw { float d[8]; uint2 y; unsigned e, bits; };
+template <typename T, int RELU, bool VEC> __device__ __forceinline__ void bn_read(const BnArgs& a, long row, int c0, int left, BnRaw& r) {
     const T* d = (const T*)a.dout + row * a.dout_ld + c0;
-    if (VEC && left >= 8) load8<T>(d, dh);
-    else load8_some<T>(d, left, dh);
-    const uint2 w = *reinterpret_cast<const uint2*>(a.y + row * a.y_ld + c0);
-    const float s = scale_value(a.y_scales[row * a.s_ld + (c0 >> 5)]);
-    float y[8];
-    decode4_e4m3(w.x, s, y);
-    decode4_e4m3(w.y, s, y + 4);
-    unsigned bits = 0xff;
+    if (VEC && left >= 8) load8<T>(d, r.d);
+    else load8_some<T>(d, left, r.d);
+    r.y = *reinterpret_cast<const uint2*>(a.y + row * a.y_ld + c0);
+    r.e = a.y_scales[row * a.s_ld + (c0 >> 5)];
+    r.bits = 0xff;
     if (RELU == 3) {
         const uint8_t* m = a.mask + row * a.mask_ld;
-        if (sizeof(T) == 2) bits = m[c0 >> 3];
-        else bits = (m[c0 >> 2] & 15u) | (left > 4 ? (unsigned)m[(c0 >> 2) + 1] << 4 : 0u);
+        if (sizeof(T) == 2) r.bits = m[c0 >> 3];
+        else r.bits = (m[c0 >> 2] & 15u) | (left > 4 ? (unsigned)m[(c0 >> 2) + 1] << 4 : 0u);
     }
+}
+template <int RELU> __device__ __forceinline__ void bn_terms(const BnRaw& r, const float* mean, const float* sc, const float* sh, float* dh, float* t) {
+    const float s = scale_value(r.e);
+    float y[8];
+    decode4_e4m3(r.y.x, s, y);
+    decode4_e4m3(r.y.y, s, y + 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+        dh[i] = r.d[i];
         if (RELU == 2) dh[i] = fmaf(sc[i], y[i], sh[i]) > 0.f ? dh[i] : 0.f;
-        if (RELU == 3) dh[i] = (bits >> i) & 1 ? dh[i] : 0.f;
+        if (RELU == 3) dh[i] = (r.bits >> i) & 1 ? dh[i] : 0.f;
         t[i] = y[i] - mean[i];
     }
 }
@@ -206,14 +213,29 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
         sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
         sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
     }
-    const long r1 = min(a.rows, (long)(blockIdx.x + 1) * a.strip);
-    if (left > 0)
-        for (long r = (long)blockIdx.x * a.strip + rg; r < r1; r += groups) {
-            float dh[8], t[8];
-            bn_chunk<T, RELU, VEC>(a, r, c0, left, mean, sc, sh, dh, t);
+    auto add = [&](const BnRaw& raw) {
+        float dh[8], t[8];
+        bn_terms<RELU>(raw, mean, sc, sh, dh, t);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { s1[i] += dh[i]; s2[i] = fmaf(dh[i], t[i], s2[i]); }
+        for (int i = 0; i < 8; ++i) { s1[i] += dh[i]; s2[i] = fmaf(dh[i], t[i], s2[i]); }
+    };
+    if (left > 0) {
+        for (long r = (long)blockIdx.x * BN_ROWS * groups + rg; r < a.rows; r += (long)a.strips * BN_ROWS * groups) {
+            if (r + (BN_ROWS - 1) * groups < a.rows) {
+                BnRaw raw[BN_ROWS];
+#pragma unroll
+                for (int k = 0; k < BN_ROWS; ++k) bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw[k]);
+#pragma unroll
+                for (int k = 0; k < BN_ROWS; ++k) add(raw[k]);
+            } else {
+                for (int k = 0; k < BN_ROWS && r + k * groups < a.rows; ++k) {
+                    BnRaw raw;
+                    bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw);
+                    add(raw);
+                }
+            }
         }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) red[threadIdx.x][i] = make_float2(s1[i], s2[i]);
     __syncthreads();
@@ -237,12 +259,12 @@ __global__ __launch_bounds__(256) void bn_finish_kernel(BnArgs a) {
     double2 s = make_double2(0.0, 0.0);
     if (ch < a.C) {
         int i = k;
-        for (; i + 3 * SLICES < a.strips; i += 4 * SLICES) {
-            double2 v[4];
+        for (; i + 7 * SLICES < a.strips; i += 8 * SLICES) {
+            double2 v[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = a.part[(long)(i + u * SLICES) * a.C + ch];
+            for (int u = 0; u < 8; ++u) v[u] = a.part[(long)(i + u * SLICES) * a.C + ch];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) { s.x += v[u].x; s.y += v[u].y; }
+            for (int u = 0; u < 8; ++u) { s.x += v[u].x; s.y += v[u].y; }
         }
         for (; i < a.strips; i += SLICES) {
             const double2 v = a.part[(long)i * a.C + ch];
@@ -280,10 +302,9 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
         sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
         sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
     }
-    const long r1 = min(a.rows, (long)(blockIdx.x + 1) * a.strip);
-    for (long r = (long)blockIdx.x * a.strip + rg; r < r1; r += groups) {
+    auto write = [&](long r, const BnRaw& raw) {
         float dh[8], t[8];
-        bn_chunk<T, RELU, VEC>(a, r, c0, left, mean, sc, sh, dh, t);
+        bn_terms<RELU>(raw, mean, sc, sh, dh, t);
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = fmaf(ga[i], dh[i], fmaf(c2[i], t[i], c1[i]));
         T* o = (T*)a.dy + r * a.dy_ld + c0;
@@ -301,10 +322,25 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
         }
         if (VEC && left >= 8) store8<T>(o, t);
         else store8_some<T>(o, left, t);
+    };
+    for (long r = (long)blockIdx.x * BN_APPLY_ROWS * groups + rg; r < a.rows; r += (long)gridDim.x * BN_APPLY_ROWS * groups) {
+        if (r + (BN_APPLY_ROWS - 1) * groups < a.rows) {               // (all the rows' loads before the first store: the outputs may be dout itself)
+            BnRaw raw[BN_APPLY_ROWS];
+#pragma unroll
+            for (int k = 0; k < BN_APPLY_ROWS; ++k) bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw[k]);
+#pragma unroll
+            for (int k = 0; k < BN_APPLY_ROWS; ++k) write(r + k * groups, raw[k]);
+        } else {
+            for (int k = 0; k < BN_APPLY_ROWS && r + k * groups < a.rows; ++k) {
+                BnRaw raw;
+                bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw);
+                write(r + k * groups, raw);
+            }
+        }
     }
 }
 
-struct BnPlan { int cols_log2, ctiles, strips; long strip; };
+struct BnPlan { int cols_log2, ctiles, strips, apply_strips; };
 BnPlan bn_plan(int64_t rows, int C) {
     BnPlan p;
     const int chunks = (C + 7) / 8;
@@ -312,21 +348,20 @@ BnPlan bn_plan(int64_t rows, int C) {
     while ((1 << p.cols_log2) < chunks && (1 << p.cols_log2) < BN_COLS) ++p.cols_log2;
     p.ctiles = (chunks + (1 << p.cols_log2) - 1) >> p.cols_log2;
     const int groups = THREADS >> p.cols_log2;
-    // about 1024 blocks in all, at least four rows per thread
-    long strips = 1024 / p.ctiles, most = (rows + groups * 4 - 1) / (groups * 4);
-    if (strips > most) strips = most;
-    if (strips < 1) strips = 1;
-    p.strip = (rows + strips - 1) / strips;
-    p.strip = (p.strip + groups - 1) / groups * groups;
-    p.strips = (int)((rows + p.strip - 1) / p.strip);
+    auto strips = [&](long blocks, int each) {
+        const long most = (rows + groups * each - 1) / (groups * each), n = blocks / p.ctiles;
+        return (int)(n > most ? most : n < 1 ? 1 : n);
+    };
+    p.strips = strips(BN_BLOCKS, BN_ROWS);
+    p.apply_strips = strips(BN_APPLY_BLOCKS, BN_APPLY_ROWS);
     return p;
 }
 
 template <typename T, int RELU> void bn_launch(const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
-    const dim3 grid(p.strips, p.ctiles);
+    const dim3 grid(p.strips, p.ctiles), apply_grid(p.apply_strips, p.ctiles);
     hipLaunchKernelGGL((vec ? bn_reduce_kernel<T, RELU, true> : bn_reduce_kernel<T, RELU, false>), grid, dim3(THREADS), 0, st, a);
     hipLaunchKernelGGL(bn_finish_kernel, dim3((a.C + FIN - 1) / FIN), dim3(THREADS), 0, st, a);
-    hipLaunchKernelGGL((vec ? bn_apply_kernel<T, RELU, true> : bn_apply_kernel<T, RELU, false>), grid, dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((vec ? bn_apply_kernel<T, RELU, true> : bn_apply_kernel<T, RELU, false>), apply_grid, dim3(THREADS), 0, st, a);
 }
 template <typename T> void bn_by_relu(int relu, const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
     if (relu == 0) bn_launch<T, 0>(a, p, vec, st);
@@ -368,7 +403,7 @@ extern "C" int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream) {
     a.dgamma = d->dgamma; a.dbeta = d->dbeta; a.dy = d->dy; a.dres = d->dres;
     a.coef = (float4*)d->ws; a.part = (double2*)((char*)d->ws + (int64_t)d->C * 16);
     a.dout_ld = d->dout_ld; a.y_ld = d->y_ld; a.s_ld = d->s_ld; a.mask_ld = d->mask_ld; a.dy_ld = d->dy_ld; a.dres_ld = d->dres_ld;
-    a.rows = d->rows; a.strip = p.strip; a.C = d->C; a.strips = p.strips; a.cols_log2 = p.cols_log2; a.accumulate = d->accumulate; a.dres_acc = d->dres_acc;
+    a.rows = d->rows; a.C = d->C; a.strips = p.strips; a.cols_log2 = p.cols_log2; a.accumulate = d->accumulate; a.dres_acc = d->dres_acc;
     const bool vec = vec_ok(d->dout, d->dout_ld, d->dtype) && vec_ok(d->dy, d->dy_ld, d->dtype) && (!d->dres || vec_ok(d->dres, d->dres_ld, d->dtype));
     hipStream_t st = (hipStream_t)stream;
     if (d->dtype == MSC_F32) bn_by_relu<float>(d->relu, a, p, vec, st);

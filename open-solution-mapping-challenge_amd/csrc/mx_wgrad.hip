@@ -58,7 +58,7 @@ template <typename T, int UPR> __device__ __forceinline__ void stage_q(char* row
         w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
         e = 127;
     }
-    const float s = pow2_field(e);
+    const float s = pow2_field(max(e, 1u));                            // 0: a pixel that was not read
     const unsigned c[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 2) {
         unsigned o[8];
@@ -85,73 +85,114 @@ template <typename T, int UPR> __device__ __forceinline__ void stage_q(char* row
     }
 }
 
-template <typename T, int TA, int TB, bool VECP> __global__ __launch_bounds__(THREADS, 2) void mx_wgrad_kernel(WgArgs a) {
+template <typename T, int TA, int TB, int KG, bool VECP> __global__ __launch_bounds__(KG * THREADS, 2) void mx_wgrad_kernel(WgArgs a) {
     using L = Tile<T, TA, TB>;
     constexpr int UPRA = L::PITCH_A / 16, UPRB = L::PITCH_B / 16;
-    __shared__ __attribute__((aligned(16))) char smem[2 * L::STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    static_assert(KG == 1 || 2 * L::STAGE >= L::NF * THREADS * 16, "a group's sums fit its stages");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int grp = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, lane = tid & 63, wid = tid >> 6;
+    char* const smem = lds + grp * 2 * L::STAGE;
     const int wa = wid >> 1, wb = wid & 1, g = lane >> 4, pl = lane & 15;
-    // consecutive blocks: the tiles of one tap and one pixel range, then the taps, then the ranges -- what runs together reads the same pixels
-    const unsigned bt = div_of(blockIdx.x, a.tile_div);
-    const int tile = (int)(blockIdx.x - bt * a.tile_div.d);
+    // order: the tiles of one tap and one pixel range, then the taps, then the ranges.  Block b runs on XCD b % 8.  Where a few blocks read the same pixels each XCD
+    // gets a run of the order, so that they share an L2 (131072 pixels, 256 x 64, two tiles: 16.5 us against 17.8); where many do, they are spread over the
+    // XCDs: the same lines wanted by 36 blocks of one XCD at a time make a queue (32x16x16, 256 -> 256, 3x3: 29.4 us against 25.4)
+    const unsigned xcd = blockIdx.x & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
+    const unsigned id = a.tiles * a.taps <= 8 ? xcd * per + min(xcd, more) + (blockIdx.x >> 3) : blockIdx.x;
+    const unsigned bt = div_of(id, a.tile_div);
+    const int tile = (int)(id - bt * a.tile_div.d);
     const int split = (int)(bt / (unsigned)a.taps), tap = (int)(bt - (unsigned)split * a.taps);
     const int a0 = tile / a.tiles_b * TA, b0 = tile % a.tiles_b * TB;
     const int kh = tap / a.KW, kw = tap - kh * a.KW;
-    const int mbeg = split * a.chunk, mend = min(a.M, mbeg + a.chunk);
-    const int steps = (mend - mbeg + L::KP - 1) / L::KP;
+    const int beg = split * a.chunk, mend = min(a.M, beg + a.chunk), mbeg = beg + grp * L::KP;      // the groups take turns: step i of group j is pixels KP * (KG i + j) on
+    const int steps = (mend - beg + KG * L::KP - 1) / (KG * L::KP);
 
-    uint4 rp[L::IA], rq[L::IB];
-    unsigned re[L::IB];
-    auto fetch = [&](int s) {
-        const int m0 = mbeg + s * L::KP;
+    struct Regs { uint4 p[L::IA], q[L::IB]; unsigned e[L::IB]; };      // what a thread moves in one step
+    Regs even, odd;
+    // Addresses.  The descriptors' bases move with the step (scalar), the lanes' offsets into them stay: p's rows are equally far apart, and rows past the range or
+    // channels past the end read as zeros by the descriptor's extent.  q's pixel of a row, under this block's tap, advances by constants with one wrap
+    // per axis; pixels outside the image read as zeros by an offset out of range.  (Divisions and 64-bit products per load and step took more issue slots
+    // than the matrix instructions.)
+    unsigned po[L::IA];
 #pragma unroll
-        for (int i = 0; i < L::IA; ++i) {
-            const int idx = i * THREADS + tid, m = m0 + idx / L::UA, c = a0 + idx % L::UA * L::PE;
-            const T* src = (const T*)a.p + (long)m * a.p_ld + c;
-            rp[i] = make_uint4(0, 0, 0, 0);
-            if (m < mend) {
-                if (VECP) {
-                    if (c < a.A) rp[i] = *reinterpret_cast<const uint4*>(src);          // A is a whole number of units
-                } else {
-                    unsigned t[4] = {0, 0, 0, 0};
+    for (int i = 0; i < L::IA; ++i) {
+        const int idx = i * THREADS + tid, c = idx % L::UA * L::PE;
+        po[i] = a0 + c < a.A ? (unsigned)(idx / L::UA) * (unsigned)(a.p_ld * L::ES) + c * L::ES : OOB_OFF;
+    }
+    const char* const pbase = a.p + ((long)mbeg * a.p_ld + a0) * L::ES;
+    const unsigned first_n = div_of((unsigned)beg, a.hw);
+    const long first_pix = a.direct ? beg : (long)first_n * a.Hq * a.Wq;
+    const int pixels = a.direct ? mend - beg : (int)(div_of((unsigned)(mend - 1), a.hw) - first_n + 1) * a.Hq * a.Wq;
+    const __amdgpu_buffer_rsrc_t rq_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + first_pix * a.q_ld), 0, (int)((pixels - 1) * a.q_ld + a.q_bytes), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.qs + first_pix * a.s_ld), 0, (int)((pixels - 1) * a.s_ld + a.q_bytes / BLOCK), 0x00020000);
+    int qrow[L::IB], qx[L::IB], qy[L::IB], qpix[L::IB], qb[L::IB];
+#pragma unroll
+    for (int i = 0; i < L::IB; ++i) {
+        const int idx = i * THREADS + tid, row = idx / L::UB;
+        const unsigned m = (unsigned)(mbeg + row), n = div_of(m, a.hw), rem = m - n * a.hw.d, y = div_of(rem, a.w);
+        qb[i] = b0 + idx % L::UB * 16;
+        qrow[i] = qb[i] < a.q_bytes && !(L::B_SOME && idx >= L::KP * L::UB) ? row : 0x7fffffff;
+        qy[i] = (int)y;
+        qx[i] = (int)(rem - y * a.w.d);
+        qpix[i] = a.direct ? grp * L::KP + row : ((int)(n - first_n) * a.Hq + qy[i] * a.stride - a.pad + kh) * a.Wq + qx[i] * a.stride - a.pad + kw;
+    }
+    const int Hp = (int)(a.hw.d / a.w.d), Wp = (int)a.w.d;
+    const int dn = (int)div_of(KG * L::KP, a.hw), dr = KG * L::KP - dn * (int)a.hw.d, dy = (int)div_of((unsigned)dr, a.w), dx = dr - dy * Wp;
+    const int dpix = a.direct ? KG * L::KP : (dn * a.Hq + dy * a.stride) * a.Wq + dx * a.stride;
+    const int wrap_x = a.direct ? 0 : (a.Wq - Wp) * a.stride, wrap_y = a.direct ? 0 : (a.Hq - Hp * a.stride) * a.Wq;
+    // output rows / columns whose pixel under this tap is inside the image: [lo, lo + n)
+    auto first_in = [&](int k) { return (max(a.pad - k, 0) + a.stride - 1) / a.stride; };
+    auto end_in = [&](int k, int in, int out) { return min(out, (in - 1 + a.pad - k) / a.stride + 1); };
+    const int ylo = a.direct ? 0 : first_in(kh), yn = a.direct ? Hp : (a.Hq - 1 + a.pad - kh < 0 ? 0 : max(0, end_in(kh, a.Hq, Hp) - ylo));
+    const int xlo = a.direct ? 0 : first_in(kw), xn = a.direct ? Wp : (a.Wq - 1 + a.pad - kw < 0 ? 0 : max(0, end_in(kw, a.Wq, Wp) - xlo));
+    auto fetch = [&](int s, Regs& r) {                                 // in the order of the steps
+        const int left = mend - mbeg - s * KG * L::KP;                 // rows; the last group's may be none
+        const char* const at = pbase + (long)s * (KG * L::KP) * a.p_ld * L::ES;
+        if constexpr (VECP) {
+            const __amdgpu_buffer_rsrc_t rp_ = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, left > 0 ? (int)(((min(left, L::KP) - 1) * a.p_ld + a.A - a0) * L::ES) : 0, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < L::IA; ++i) r.p[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rp_, (int)po[i], 0, 0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::IA; ++i) {
+                const int idx = i * THREADS + tid, row = idx / L::UA, c = a0 + idx % L::UA * L::PE;
+                const char* src = at + (long)row * a.p_ld * L::ES + idx % L::UA * 16;
+                unsigned t[4] = {0, 0, 0, 0};
+                if (row < left)
 #pragma unroll
                     for (int k = 0; k < L::PE; ++k)
                         if (c + k < a.A) {
                             if (L::ES == 2) t[k >> 1] |= (unsigned)reinterpret_cast<const uint16_t*>(src)[k] << (k & 1) * 16;
                             else t[k & 3] = reinterpret_cast<const unsigned*>(src)[k];
                         }
-                    rp[i] = make_uint4(t[0], t[1], t[2], t[3]);
-                }
+                r.p[i] = make_uint4(t[0], t[1], t[2], t[3]);
             }
         }
 #pragma unroll
         for (int i = 0; i < L::IB; ++i) {
-            const int idx = i * THREADS + tid, m = m0 + idx / L::UB, b = b0 + idx % L::UB * 16;
-            rq[i] = make_uint4(0, 0, 0, 0);
-            re[i] = 127;
-            if (m >= mend || b >= a.q_bytes || (L::B_SOME && idx >= L::KP * L::UB)) continue;
-            long at = m;
-            if (!a.direct) {
-                const unsigned n = div_of((unsigned)m, a.hw), rem = (unsigned)m - n * a.hw.d, y = div_of(rem, a.w), x = rem - y * a.w.d;
-                const int iy = (int)y * a.stride - a.pad + kh, ix = (int)x * a.stride - a.pad + kw;
-                if ((unsigned)iy >= (unsigned)a.Hq || (unsigned)ix >= (unsigned)a.Wq) continue;
-                at = ((long)n * a.Hq + iy) * a.Wq + ix;
-            }
-            rq[i] = *reinterpret_cast<const uint4*>(a.q + at * a.q_ld + b);
-            re[i] = a.qs[at * a.s_ld + (b >> 5)];
+            const bool in = qrow[i] < left && (unsigned)(qy[i] - ylo) < (unsigned)yn && (unsigned)(qx[i] - xlo) < (unsigned)xn;
+            r.q[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq_, in ? qpix[i] * (int)a.q_ld + qb[i] : (int)OOB_OFF, 0, 0));
+            r.e[i] = __builtin_amdgcn_raw_buffer_load_b8(rs_, in ? qpix[i] * (int)a.s_ld + (qb[i] >> 5) : (int)OOB_OFF, 0, 0);
+            qpix[i] += dpix;
+            qx[i] += dx;
+            const bool wx = qx[i] >= Wp;
+            qx[i] -= wx ? Wp : 0;
+            qy[i] += dy + (wx ? 1 : 0);
+            const bool wy = qy[i] >= Hp;
+            qy[i] -= wy ? Hp : 0;
+            qpix[i] += (wx ? wrap_x : 0) + (wy ? wrap_y : 0);
         }
     };
-    auto put = [&](char* st) {
+    auto put = [&](char* st, const Regs& v) {
 #pragma unroll
         for (int i = 0; i < L::IA; ++i) {
             const int idx = i * THREADS + tid, r = idx / L::UA, u = idx % L::UA;
-            *reinterpret_cast<uint4*>(st + r * L::PITCH_A + (L::ES == 2 ? swz16<UPRA>(u, r) : u) * 16) = rp[i];
+            *reinterpret_cast<uint4*>(st + r * L::PITCH_A + (L::ES == 2 ? swz16<UPRA>(u, r) : u) * 16) = v.p[i];
         }
         char* sq = st + L::KP * L::PITCH_A;
 #pragma unroll
         for (int i = 0; i < L::IB; ++i) {
             const int idx = i * THREADS + tid, r = idx / L::UB, u = idx % L::UB;
-            if (!L::B_SOME || idx < L::KP * L::UB) stage_q<T, UPRB>(sq + r * L::PITCH_B, u, r, rq[i], re[i]);
+            if (!L::B_SOME || idx < L::KP * L::UB) stage_q<T, UPRB>(sq + r * L::PITCH_B, u, r, v.q[i], v.e[i]);
         }
     };
 
@@ -204,16 +245,42 @@ template <typename T, int TA, int TB, bool VECP> __global__ __launch_bounds__(TH
         }
     };
 
-    fetch(0);
-    put(smem);
+    // two steps' loads are in flight in registers while a third is multiplied
+    fetch(0, even);
+    if (steps > 1) fetch(1, odd);
+    put(smem, even);
+    if (steps > 2) fetch(2, even);
     __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) fetch(s + 1);
+    auto step = [&](int s, Regs& r) {                                  // r: step s + 1, which goes to the half last read two barriers ago
         compute(smem + (s & 1) * L::STAGE);
-        if (s + 1 < steps) put(smem + ((s + 1) & 1) * L::STAGE);      // last read two barriers ago
+        if (s + 1 < steps) put(smem + ((s + 1) & 1) * L::STAGE, r);
+        if (s + 3 < steps) fetch(s + 3, r);
         __syncthreads();
+    };
+    for (int s = 0; s < steps; s += 2) {
+        step(s, odd);
+        if (s + 1 < steps) step(s + 1, even);
     }
 
+    if constexpr (KG > 1) {              // the groups' sums, in order, through the stages that were multiplied last
+        float4* mine = reinterpret_cast<float4*>(smem) + tid;
+        if (grp) {
+#pragma unroll
+            for (int f = 0; f < L::NF; ++f) {
+                const f32x4 v = acc[f / L::FN][f % L::FN];
+                mine[f * THREADS] = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k)
+#pragma unroll
+            for (int f = 0; f < L::NF; ++f) {
+                const float4 v = reinterpret_cast<const float4*>(lds + k * 2 * L::STAGE)[f * THREADS + tid];
+                acc[f / L::FN][f % L::FN] += f32x4{v.x, v.y, v.z, v.w};
+            }
+    }
     // a lane holds, of fragment (i, j): b = b0 + half + 16 j + 4 g + 0..3, a = a0 + half + 16 i + pl
     if (a.splits > 1) {
         float4* o = reinterpret_cast<float4*>(a.part) + ((long)(split * a.taps + tap) * a.tiles + tile) * (L::NF * THREADS) + tid;
@@ -235,26 +302,39 @@ template <typename T, int TA, int TB, bool VECP> __global__ __launch_bounds__(TH
     }
 }
 
-// adds the ranges' partial tiles in order; one float4 per thread, at the place the tile kernel's thread wrote it
-template <int TA, int TB> __global__ __launch_bounds__(THREADS) void mx_wgrad_join_kernel(WgArgs a) {
-    constexpr int FN = TB / 32, NF = TA / 32 * FN;
-    const int bt = blockIdx.x / NF, f = blockIdx.x % NF, tap = bt / a.tiles, tile = bt % a.tiles;
+// adds the ranges' partial tiles, SLICES of them side by side (a fixed order); a float4 per thread, at the places the tile kernel's threads wrote
+template <int TA, int TB, int SLICES> __global__ __launch_bounds__(THREADS) void mx_wgrad_join_kernel(WgArgs a) {
+    constexpr int FN = TB / 32, NF = TA / 32 * FN, PLACES = THREADS / SLICES;
+    __shared__ float4 red[SLICES > 1 ? THREADS : 1];
+    const int slice = threadIdx.x / PLACES;
+    const long at = (long)blockIdx.x * PLACES + threadIdx.x % PLACES;                  // [tap][tile][fragment][thread of the tile kernel]
     const long plane = (long)a.taps * a.tiles * NF * THREADS;
-    const float4* src = reinterpret_cast<const float4*>(a.part) + ((long)bt * NF + f) * THREADS + threadIdx.x;
+    const float4* src = reinterpret_cast<const float4*>(a.part) + at;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    int k = 0;
-    for (; k + 8 <= a.splits; k += 8) {
+    int k = slice;
+    for (; k + 7 * SLICES < a.splits; k += 8 * SLICES) {
         float4 v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = src[(k + i) * plane];
+        for (int i = 0; i < 8; ++i) v[i] = src[(k + i * SLICES) * plane];
 #pragma unroll
         for (int i = 0; i < 8; ++i) { s.x += v[i].x; s.y += v[i].y; s.z += v[i].z; s.w += v[i].w; }
     }
-    for (; k < a.splits; ++k) {
+    for (; k < a.splits; k += SLICES) {
         const float4 v = src[k * plane];
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    if constexpr (SLICES > 1) {
+        red[threadIdx.x] = s;
+        __syncthreads();
+        if (slice) return;
+#pragma unroll
+        for (int i = 1; i < SLICES; ++i) {
+            const float4 v = red[i * PLACES + threadIdx.x];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+    }
+    const int thread = (int)(at % THREADS), f = (int)(at / THREADS % NF), bt = (int)(at / (THREADS * NF)), tap = bt / a.tiles, tile = bt % a.tiles;
+    const int lane = thread & 63, wid = thread >> 6;
     const int ia = tile / a.tiles_b * TA + (wid >> 1) * (TA / 2) + f / FN * 16 + (lane & 15);
     const int ib = tile % a.tiles_b * TB + (wid & 1) * (TB / 2) + f % FN * 16 + 4 * (lane >> 4);
     if (ia >= a.A) return;
@@ -265,7 +345,7 @@ template <int TA, int TB> __global__ __launch_bounds__(THREADS) void mx_wgrad_jo
         if (ib + i < a.B) o[i] = (a.accumulate ? o[i] : 0.f) + v[i];
 }
 
-struct WgPlan { int ta, tb, tiles_a, tiles_b, splits, chunk; };
+struct WgPlan { int ta, tb, kg, tiles_a, tiles_b, splits, chunk; };
 WgPlan wg_plan(const msc_mx_wgrad_desc* d) {
     WgPlan p;
     p.ta = d->A > 64 ? 128 : 64;
@@ -274,10 +354,17 @@ WgPlan wg_plan(const msc_mx_wgrad_desc* d) {
     p.tiles_b = (d->B + p.tb - 1) / p.tb;
     const int64_t M = (int64_t)d->N * d->Hp * d->Wp, all = (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW;
     const int kp = d->dtype == MSC_F32 ? 32 : 64;
-    int64_t splits = 512 / all, most = (M + 4 * kp - 1) / (4 * kp);       // two blocks per CU, at least four steps each
+        // two groups of waves to a block and one block to a CU where every group has four steps to do: half the partial sums of two blocks with one group each
+    // (3x3 above: 25.4 + 5.5 us to join, against 24.7 + 7.3; 1x1: 16.5 + 4.0 against 17.3 + 4.5).  Fewer pixels: more, smaller blocks
+    p.kg = M * all >= 256ll * 2 * 4 * kp ? 2 : 1;
+    int64_t splits = 512 / p.kg / all, most = (M + 4 * p.kg * kp - 1) / (4 * p.kg * kp);
     if (splits > most) splits = most;
+    // a block's offsets into q are 32-bit: its images, one more at each end, stay below 1 GiB (a single image does, wg_check)
+    const int64_t image = (int64_t)d->Hq * d->Wq * (d->q_ld > d->s_ld ? d->q_ld : d->s_ld), hw = (int64_t)d->Hp * d->Wp;
+    const int64_t images = (1ll << 30) / (image > 1 ? image : 1), pixels = (images > 3 ? images - 2 : 1) * hw;
+    if (splits < (M + pixels - 1) / pixels) splits = (M + pixels - 1) / pixels;
     if (splits < 1) splits = 1;
-    p.chunk = (int)(((M + splits - 1) / splits + kp - 1) / kp * kp);
+    p.chunk = (int)(((M + splits - 1) / splits + p.kg * kp - 1) / (p.kg * kp) * (p.kg * kp));
     p.splits = (int)((M + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -291,20 +378,36 @@ int wg_check(const msc_mx_wgrad_desc* d) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: kernel %dx%d, stride %d, padding %d", d->KH, d->KW, d->stride, d->pad);
     if ((int64_t)d->N * d->Hp * d->Wp >= 1ll << 30 || (int64_t)d->Hq * d->Wq >= 1ll << 30)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 pixels or more");
+    if ((int64_t)d->Hq * d->Wq * d->q_ld >= 1ll << 28 || (int64_t)d->Hq * d->Wq * d->s_ld >= 1ll << 28 || d->p_ld >= 1ll << 24)
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: an image of 2^28 bytes of codes or more, or rows of 2^24 elements");
     return MSC_OK;
 }
 
-template <typename T, int TA, int TB> void wg_launch(const WgArgs& a, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)(a.tiles * a.taps * a.splits));
-    hipLaunchKernelGGL((vec ? mx_wgrad_kernel<T, TA, TB, true> : mx_wgrad_kernel<T, TA, TB, false>), grid, dim3(THREADS), 0, st, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL((mx_wgrad_join_kernel<TA, TB>), dim3((unsigned)(a.tiles * a.taps * (TA / 32) * (TB / 32))), dim3(THREADS), 0, st, a);
+template <typename T, int TA, int TB, int KG> int wg_launch_tiles(const WgArgs& a, bool vec, hipStream_t st) {
+    constexpr int LDS = KG * 2 * Tile<T, TA, TB>::STAGE;
+    auto k = vec ? mx_wgrad_kernel<T, TA, TB, KG, true> : mx_wgrad_kernel<T, TA, TB, KG, false>;
+    if (LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return msc_fail(MSC_ERR_HIP, "msc_mx_wgrad: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)(a.tiles * a.taps * a.splits)), dim3(KG * THREADS), LDS, st, a);
+    return MSC_OK;
 }
-template <typename T> void wg_by_tile(const WgPlan& p, const WgArgs& a, bool vec, hipStream_t st) {
-    if (p.ta == 128 && p.tb == 128) wg_launch<T, 128, 128>(a, vec, st);
-    else if (p.ta == 128) wg_launch<T, 128, 64>(a, vec, st);
-    else if (p.tb == 128) wg_launch<T, 64, 128>(a, vec, st);
-    else wg_launch<T, 64, 64>(a, vec, st);
+template <typename T, int TA, int TB> int wg_launch(const WgPlan& p, const WgArgs& a, bool vec, hipStream_t st) {
+    const int rc = p.kg == 2 ? wg_launch_tiles<T, TA, TB, 2>(a, vec, st) : wg_launch_tiles<T, TA, TB, 1>(a, vec, st);
+    if (rc || a.splits == 1) return rc;
+    const int64_t places = (int64_t)a.tiles * a.taps * TA * TB / 4;
+    // enough threads to have the partial sums' reads in flight (256 ranges of 256 x 64: 12.7 us with one slice, 4.5 with sixteen)
+    if (places * 4 > 256 * THREADS || a.splits < 8) hipLaunchKernelGGL((mx_wgrad_join_kernel<TA, TB, 1>), dim3((unsigned)(places / THREADS)), dim3(THREADS), 0, st, a);
+    else if (places * 16 > 256 * THREADS || a.splits < 32) hipLaunchKernelGGL((mx_wgrad_join_kernel<TA, TB, 4>), dim3((unsigned)(places / THREADS * 4)), dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((mx_wgrad_join_kernel<TA, TB, 16>), dim3((unsigned)(places / THREADS * 16)), dim3(THREADS), 0, st, a);
+    return MSC_OK;
+}
+template <typename T> int wg_by_tile(const WgPlan& p, const WgArgs& a, bool vec, hipStream_t st) {
+    if (p.ta == 128 && p.tb == 128) return wg_launch<T, 128, 128>(p, a, vec, st);
+    if (p.ta == 128) return wg_launch<T, 128, 64>(p, a, vec, st);
+    if (p.tb == 128) return wg_launch<T, 64, 128>(p, a, vec, st);
+    return wg_launch<T, 64, 64>(p, a, vec, st);
 }
 
 }  // namespace
@@ -330,8 +433,9 @@ extern "C" int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: q needs 16-byte aligned rows of whole E4M3 blocks and one scale byte per block");
     const WgPlan p = wg_plan(d);
     if (p.splits > 1 && (!d->ws || (uintptr_t)d->ws & 15)) return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: workspace missing or not 16-byte aligned");
-    if ((int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * (p.ta / 32) * (p.tb / 32) >= 1ll << 30)
-        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: gradient of more than 2^40 elements");
+    if ((int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * (p.ta / 32) * (p.tb / 32) >= 1ll << 30 ||
+        (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * p.splits >= 1ll << 30)
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 tiles or more");
     WgArgs a;
     a.p = (const char*)d->p; a.q = d->q; a.qs = d->q_scales; a.dw = d->dw; a.part = (float*)d->ws;
     a.p_ld = d->p_ld; a.q_ld = d->q_ld; a.s_ld = d->s_ld;
@@ -342,8 +446,6 @@ extern "C" int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream) {
     a.direct = a.taps == 1 && d->stride == 1 && d->pad == 0 && d->Hq == d->Hp && d->Wq == d->Wp;
     const bool vec = vec_ok(d->p, d->p_ld, d->dtype) && d->A % msc_dtype_vec(d->dtype) == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (d->dtype == MSC_F32) wg_by_tile<float>(p, a, vec, st);
-    else if (d->dtype == MSC_BF16) wg_by_tile<bf16_t>(p, a, vec, st);
-    else wg_by_tile<f16_t>(p, a, vec, st);
-    return msc_check_launch("msc_mx_wgrad");
+    rc = d->dtype == MSC_F32 ? wg_by_tile<float>(p, a, vec, st) : d->dtype == MSC_BF16 ? wg_by_tile<bf16_t>(p, a, vec, st) : wg_by_tile<f16_t>(p, a, vec, st);
+    return rc ? rc : msc_check_launch("msc_mx_wgrad");
 }

@@ -29,7 +29,10 @@ class MxTensor:
     Rows of codes start on 16 bytes; both may be slices of wider buffers."""
     __slots__ = ('codes', 'scales', 'channels', 'fmt')
 
-    def __init__(self, codes, scales, channels, fmt='e4m3'):
+    def __init__(self, codes, scales, channels, fmt='e4m3', check=True):
+        self.codes, self.scales, self.channels, self.fmt = codes, scales, channels, fmt
+        if not check:
+            return
         if fmt not in FORMATS:
             raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
         nb = (channels + 31) // 32
@@ -40,11 +43,10 @@ class MxTensor:
                              % (channels, fmt, nb * FORMATS[fmt][1], nb, tuple(codes.shape), tuple(scales.shape)))
         if codes.device != scales.device:
             raise ValueError('codes and scales are on different devices')
-        self.codes, self.scales, self.channels, self.fmt = codes, scales, channels, fmt
 
     @property
     def shape(self):
-        return tuple(self.codes.shape[:-1]) + (self.channels,)
+        return self.codes.shape[:-1] + (self.channels,)
 
     @property
     def device(self):
@@ -61,9 +63,10 @@ def _rows(t, what):
         raise _lib.MscError('%s: needs a CUDA/ROCm tensor; there is no CPU path in the product' % what)
     if t.dim() < 2:
         raise ValueError('%s: expected [..., channels], got shape %s' % (what, tuple(t.shape)))
+    shape = t.shape
     if t.is_contiguous():
-        return t.numel() // t.shape[-1] if t.shape[-1] else 0, t.shape[-1]
-    shape, stride = t.shape, t.stride()
+        return t.numel() // shape[-1] if shape[-1] else 0, shape[-1]
+    stride = t.stride()
     if shape[-1] > 1 and stride[-1] != 1:
         raise ValueError('%s: channels have to be next to each other (strides %s)' % (what, tuple(stride)))
     pitch, rows = None, 1
@@ -99,26 +102,29 @@ def _vector(t, n, dev, what):
 
 
 def _out(out, shape, dtype, dev, what):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev:
         raise ValueError('%s: out has to be %s %s on %s' % (what, tuple(shape), dtype, dev))
     return out
 
 
 def _run(name, dev, *args):
-    """one C call on `dev`'s current stream, with `dev` current"""
+    """one C call on `dev`'s current stream, with `dev` current.  (The stream's handle alone: the Stream object that torch.cuda.current_stream() makes
+    costs as much host time as a launch.)"""
+    fn = getattr(_lib.load(), name)
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    # the handle alone: the Stream object that torch.cuda.current_stream() makes costs as much as a launch's own host time
-    _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _workspace(name, nbytes, dev):
+def _workspace(nbytes, like, name):
+    """scratch of one call on like's device; None where it needs none"""
     if nbytes < 0:
         _lib.check(-1, name)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def empty(shape, fmt='e4m3', device='cuda'):
@@ -135,23 +141,38 @@ def pack(x, fmt='e4m3', out=None):
     if fmt not in FORMATS:
         raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
     rows, ld = _rows(x, 'pack')
-    dt = _dtype(x, 'pack')
+    dt, shape, dev = _dtype(x, 'pack'), x.shape, x.device
+    c = shape[-1]
+    fid, nbytes = FORMATS[fmt]
     if out is None:
-        out = empty(x.shape, fmt, x.device)
-    elif out.shape != tuple(x.shape) or out.fmt != fmt:
-        raise ValueError('pack: out holds %s in %s, not %s in %s' % (out.shape, out.fmt, tuple(x.shape), fmt))
-    _same_device('pack', x.device, out.codes)
-    _run('msc_mx_pack', x.device, x.data_ptr(), ld, dt, out.codes.data_ptr(), _rows(out.codes, 'pack')[1], out.scales.data_ptr(),
-         _rows(out.scales, 'pack')[1], FORMATS[fmt][0], rows, x.shape[-1])
+        if c <= 0:
+            raise ValueError('pack: no channels')
+        nb = (c + 31) // 32
+        c_ld, s_ld = nb * nbytes, nb
+        codes = torch.empty(shape[:-1] + (c_ld,), dtype=torch.uint8, device=dev)
+        scales = codes.new_empty(shape[:-1] + (nb,))
+        out = MxTensor(codes, scales, c, fmt, False)
+    else:
+        if out.shape != tuple(shape) or out.fmt != fmt:
+            raise ValueError('pack: out holds %s in %s, not %s in %s' % (out.shape, out.fmt, tuple(shape), fmt))
+        codes, scales = out.codes, out.scales
+        _same_device('pack', dev, codes)
+        c_ld, s_ld = _rows(codes, 'pack')[1], _rows(scales, 'pack')[1]
+    _run('msc_mx_pack', dev, x.data_ptr(), ld, dt, codes.data_ptr(), c_ld, scales.data_ptr(), s_ld, fid, rows, c)
     return out
 
 
 def unpack(t, dtype=torch.bfloat16, out=None):
     """the values an MxTensor stands for, in `dtype` (any of the three; the one that was packed holds every value exactly)"""
-    out = _out(out, t.shape, dtype if out is None else out.dtype, t.device, 'unpack')
-    rows, ld = _rows(out, 'unpack')
-    _run('msc_mx_unpack', t.device, t.codes.data_ptr(), _rows(t.codes, 'unpack')[1], t.scales.data_ptr(), _rows(t.scales, 'unpack')[1], FORMATS[t.fmt][0],
-         out.data_ptr(), ld, _dtype(out, 'unpack'), rows, t.channels)
+    codes, scales, dev = t.codes, t.scales, t.codes.device
+    rows, c_ld = _rows(codes, 'unpack')
+    if out is None:
+        out, ld = torch.empty(t.shape, dtype=dtype, device=dev), t.channels
+    else:
+        _out(out, t.shape, out.dtype, dev, 'unpack')
+        ld = _rows(out, 'unpack')[1]
+    _run('msc_mx_unpack', dev, codes.data_ptr(), c_ld, scales.data_ptr(), _rows(scales, 'unpack')[1], FORMATS[t.fmt][0], out.data_ptr(), ld,
+         _dtype(out, 'unpack'), rows, t.channels)
     return out
 
 
@@ -168,29 +189,29 @@ def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=
     _, q_ld = _rows(saved.codes, 'conv_weight_grad')
     _, s_ld = _rows(saved.scales, 'conv_weight_grad')
     a, b = dy.shape[-1], saved.channels
-    d = _lib.MxWgradDesc()
     if kh == 1 and kw == 1 and stride == 1 and pad == 0:
-        if tuple(dy.shape[:-1]) != saved.shape[:-1]:
-            raise ValueError('conv_weight_grad: dy %s and input %s differ in their rows' % (tuple(dy.shape), saved.shape))
-        d.N, d.Hp, d.Wp, d.Hq, d.Wq = rows, 1, 1, 1, 1
+        if dy.shape[:-1] != saved.codes.shape[:-1]:
+            raise ValueError('conv_weight_grad: dy %s and input %s differ in their rows' % (tuple(dy.shape), tuple(saved.shape)))
+        n, hp, wp, hq, wq = rows, 1, 1, 1, 1
     else:
         if dy.dim() != 4 or len(saved.shape) != 4 or dy.shape[0] != saved.shape[0]:
-            raise ValueError('conv_weight_grad: expected NHWC dy and input, got %s and %s' % (tuple(dy.shape), saved.shape))
-        (d.N, d.Hp, d.Wp), (d.Hq, d.Wq) = dy.shape[:3], saved.shape[1:3]
-        want = tuple((i + 2 * pad - k) // stride + 1 if stride > 0 else 0 for i, k in ((d.Hq, kh), (d.Wq, kw)))
-        if (d.Hp, d.Wp) != want:
-            raise ValueError('conv_weight_grad: an input of %dx%d gives an output of %dx%d, dy is %dx%d' % (d.Hq, d.Wq, want[0], want[1], d.Hp, d.Wp))
+            raise ValueError('conv_weight_grad: expected NHWC dy and input, got %s and %s' % (tuple(dy.shape), tuple(saved.shape)))
+        (n, hp, wp), (hq, wq) = dy.shape[:3], saved.shape[1:3]
+        want = tuple((i + 2 * pad - k) // stride + 1 if stride > 0 else 0 for i, k in ((hq, kh), (wq, kw)))
+        if (hp, wp) != want:
+            raise ValueError('conv_weight_grad: an input of %dx%d gives an output of %dx%d, dy is %dx%d' % (hq, wq, want[0], want[1], hp, wp))
     dev = dy.device
-    out = _out(out, (a, kh, kw, b), torch.float32, dev, 'conv_weight_grad')
-    if not out.is_contiguous():
+    if out is None:
+        out = torch.empty((a, kh, kw, b), dtype=torch.float32, device=dev)
+    elif not _out(out, (a, kh, kw, b), torch.float32, dev, 'conv_weight_grad').is_contiguous():
         raise ValueError('conv_weight_grad: out has to be contiguous')
     _same_device('conv_weight_grad', dev, saved.codes)
-    d.p, d.q, d.q_scales, d.dw = dy.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), out.data_ptr()
-    d.p_ld, d.q_ld, d.s_ld, d.dtype = p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad')
-    d.A, d.B, d.KH, d.KW, d.stride, d.pad, d.accumulate = a, b, kh, kw, stride, pad, int(accumulate)
+    d = _lib.MxWgradDesc(dy.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), out.data_ptr(), None, p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad'),
+                         n, hp, wp, a, hq, wq, b, kh, kw, stride, pad, accumulate)
     ref = C.byref(d)
-    ws = _workspace('msc_mx_wgrad_workspace_bytes', _lib.load().msc_mx_wgrad_workspace_bytes(ref), dev)
-    d.ws = None if ws is None else ws.data_ptr()
+    ws = _workspace(_lib.load().msc_mx_wgrad_workspace_bytes(ref), dy, 'msc_mx_wgrad_workspace_bytes')
+    if ws is not None:
+        d.ws = ws.data_ptr()
     _run('msc_mx_wgrad', dev, ref)
     return out
 
@@ -202,37 +223,37 @@ def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=N
     which the mask is recomputed on the stored y; or neither: no ReLU.  gamma may be None (ones).  dy may be dout (in place)."""
     if saved.fmt != 'e4m3':
         raise ValueError('batchnorm_backward: the checkpoint has to be in e4m3, got %s' % saved.fmt)
-    if tuple(dout.shape) != saved.shape:
-        raise ValueError('batchnorm_backward: dout %s and input %s differ' % (tuple(dout.shape), saved.shape))
+    if dout.shape != saved.shape:
+        raise ValueError('batchnorm_backward: dout %s and input %s differ' % (tuple(dout.shape), tuple(saved.shape)))
     if (scale is None) != (shift is None) or (scale is not None and relu_mask is not None):
         raise ValueError('batchnorm_backward: the ReLU takes relu_mask, or scale and shift, or neither')
-    dev, c = dout.device, saved.channels
-    d = _lib.MxBnBwdDesc()
-    d.rows, d.dout_ld = _rows(dout, 'batchnorm_backward')
-    _, d.y_ld = _rows(saved.codes, 'batchnorm_backward')
-    _, d.s_ld = _rows(saved.scales, 'batchnorm_backward')
-    _same_device('batchnorm_backward', dev, saved.codes, relu_mask)
-    d.dtype, d.C = _dtype(dout, 'batchnorm_backward'), c
+    dev, c, codes, scales = dout.device, saved.channels, saved.codes, saved.scales
+    rows, dout_ld = _rows(dout, 'batchnorm_backward')
+    y_ld, s_ld = _rows(codes, 'batchnorm_backward')[1], _rows(scales, 'batchnorm_backward')[1]
+    _same_device('batchnorm_backward', dev, codes, relu_mask)
+    dt, dtype = _dtype(dout, 'batchnorm_backward'), dout.dtype
+    relu, mask_ld = 0, 0
     if relu_mask is not None:
-        per = 4 if dout.dtype == torch.float32 else 8
-        if relu_mask.dtype != torch.uint8 or tuple(relu_mask.shape) != tuple(dout.shape[:-1]) + ((c + per - 1) // per,):
+        per = 4 if dt == _lib.F32 else 8
+        if relu_mask.dtype != torch.uint8 or relu_mask.shape != dout.shape[:-1] + ((c + per - 1) // per,):
             raise ValueError('batchnorm_backward: the mask has one byte for %d channels of a row, got %s %s' % (per, tuple(relu_mask.shape), relu_mask.dtype))
-        d.relu, d.relu_mask, d.mask_ld = 3, relu_mask.data_ptr(), _rows(relu_mask, 'batchnorm_backward')[1]
+        relu, mask_ld = 3, _rows(relu_mask, 'batchnorm_backward')[1]
     elif scale is not None:
-        d.relu, d.scale, d.shift = 2, _vector(scale, c, dev, 'batchnorm_backward: scale'), _vector(shift, c, dev, 'batchnorm_backward: shift')
-    d.gamma = _vector(gamma, c, dev, 'batchnorm_backward: gamma')
-    d.mean, d.invstd = _vector(mean, c, dev, 'batchnorm_backward: mean'), _vector(invstd, c, dev, 'batchnorm_backward: invstd')
-    dy = _out(dy, dout.shape, dout.dtype, dev, 'batchnorm_backward')
-    d.dy_ld = _rows(dy, 'batchnorm_backward')[1]
-    dgamma, dbeta = torch.empty((2, c), dtype=torch.float32, device=dev)
-    d.dout, d.y, d.y_scales, d.dy = dout.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), dy.data_ptr()
-    d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
-    dres = None
-    if residual:
-        dres = torch.empty(dout.shape, dtype=dout.dtype, device=dev)
-        d.dres, d.dres_ld = dres.data_ptr(), c
-    ws = _workspace('msc_mx_bn_bwd_workspace_bytes', _lib.load().msc_mx_bn_bwd_workspace_bytes(d.rows, c), dev)
-    d.ws = None if ws is None else ws.data_ptr()
+        relu = 2
+    if dy is None:
+        dy, dy_ld = torch.empty(dout.shape, dtype=dtype, device=dev), c
+    else:
+        dy_ld = _rows(_out(dy, dout.shape, dtype, dev, 'batchnorm_backward'), 'batchnorm_backward')[1]
+    dgamma = torch.empty(c, dtype=torch.float32, device=dev)
+    dbeta = dgamma.new_empty(c)
+    dres = torch.empty(dout.shape, dtype=dtype, device=dev) if residual else None
+    ws = _workspace(_lib.load().msc_mx_bn_bwd_workspace_bytes(rows, c), dout, 'msc_mx_bn_bwd_workspace_bytes')
+    d = _lib.MxBnBwdDesc(dout.data_ptr(), codes.data_ptr(), scales.data_ptr(), relu_mask.data_ptr() if relu_mask is not None else None,
+                         _vector(gamma, c, dev, 'batchnorm_backward: gamma'), _vector(mean, c, dev, 'batchnorm_backward: mean'),
+                         _vector(invstd, c, dev, 'batchnorm_backward: invstd'), _vector(scale, c, dev, 'batchnorm_backward: scale'),
+                         _vector(shift, c, dev, 'batchnorm_backward: shift'), dgamma.data_ptr(), dbeta.data_ptr(), dy.data_ptr(),
+                         dres.data_ptr() if residual else None, ws.data_ptr() if ws is not None else None, dout_ld, y_ld, s_ld, mask_ld, dy_ld, c, rows,
+                         dt, c, relu, 0, 0)
     _run('msc_mx_bn_bwd', dev, C.byref(d))
     return (dy, dgamma, dbeta, dres) if residual else (dy, dgamma, dbeta)
 
@@ -244,33 +265,35 @@ def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=N
     packed = isinstance(x, MxTensor)
     if w.fmt != 'e2m1' or (packed and x.fmt != 'e2m1'):
         raise ValueError('linear: the operands have to be in e2m1')
-    if len(w.shape) != 2 or w.channels != x.shape[-1]:
-        raise ValueError('linear: x %s and w %s do not go together' % (tuple(x.shape), w.shape))
-    dev, (n, k) = x.device, w.shape
+    wc, k = w.codes, w.channels
+    if wc.dim() != 2 or k != x.shape[-1]:
+        raise ValueError('linear: x %s and w %s do not go together' % (tuple(x.shape), tuple(w.shape)))
+    dev, n = x.device, wc.shape[0]
     if dtype is None:
-        dtype = out.dtype if out is not None else x.dtype if not packed else res.dtype if res is not None else torch.bfloat16
+        dtype = x.dtype if not packed else out.dtype if out is not None else res.dtype if res is not None else torch.bfloat16
     if not packed and x.dtype != dtype:
         raise ValueError('linear: the result has the type of x')
-    out = _out(out, tuple(x.shape[:-1]) + (n,), dtype, dev, 'linear')
-    _same_device('linear', dev, w.codes)
-    d = _lib.MxLinearDesc()
     if packed:
-        d.M, d.xc_ld = _rows(x.codes, 'linear')
-        d.x_codes, d.x_scales, d.xs_ld = x.codes.data_ptr(), x.scales.data_ptr(), _rows(x.scales, 'linear')[1]
+        m, xc_ld = _rows(x.codes, 'linear')
+        xp, x_ld, xcp, xsp, xs_ld = None, 0, x.codes.data_ptr(), x.scales.data_ptr(), _rows(x.scales, 'linear')[1]
     else:
-        d.M, d.x_ld = _rows(x, 'linear')
-        d.x = x.data_ptr()
-    d.w, d.w_scales, d.w_ld, d.s_ld = w.codes.data_ptr(), w.scales.data_ptr(), _rows(w.codes, 'linear')[1], _rows(w.scales, 'linear')[1]
-    d.scale, d.shift = _vector(scale, n, dev, 'linear: scale'), _vector(shift, n, dev, 'linear: shift')
-    if res is not None:
-        _out(res, out.shape, dtype, dev, 'linear: res')
-        d.res, d.res_ld = res.data_ptr(), _rows(res, 'linear')[1]
-    d.out, d.out_ld = out.data_ptr(), _rows(out, 'linear')[1]
-    d.dtype, d.K, d.N, d.relu = _dtype(out, 'linear'), k, n, int(relu)
-    if d.M == 0:
+        m, x_ld = _rows(x, 'linear')
+        xp, xcp, xsp, xc_ld, xs_ld = x.data_ptr(), None, None, 0, 0
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out, out_ld = torch.empty(shape, dtype=dtype, device=dev), n
+    else:
+        out_ld = _rows(_out(out, shape, dtype, dev, 'linear'), 'linear')[1]
+    _same_device('linear', dev, wc)
+    resp, res_ld = (None, 0) if res is None else (res.data_ptr(), _rows(_out(res, shape, dtype, dev, 'linear: res'), 'linear')[1])
+    if m == 0:
         return out
+    d = _lib.MxLinearDesc(xp, xcp, xsp, wc.data_ptr(), w.scales.data_ptr(), _vector(scale, n, dev, 'linear: scale'), _vector(shift, n, dev, 'linear: shift'), resp,
+                          out.data_ptr(), None, x_ld, xc_ld, xs_ld, _rows(wc, 'linear')[1], _rows(w.scales, 'linear')[1], res_ld, out_ld, m,
+                          _dtype(out, 'linear'), k, n, relu)
     ref = C.byref(d)
-    ws = _workspace('msc_mx_linear_workspace_bytes', _lib.load().msc_mx_linear_workspace_bytes(ref), dev)
-    d.ws = None if ws is None else ws.data_ptr()
+    ws = _workspace(_lib.load().msc_mx_linear_workspace_bytes(ref), wc, 'msc_mx_linear_workspace_bytes')
+    if ws is not None:
+        d.ws = ws.data_ptr()
     _run('msc_mx_linear', dev, ref)
     return out
