@@ -493,7 +493,7 @@ int msc_size_matrix(const int32_t* labels, int32_t* sizes, int32_t* areas, int B
  *   codes  : MSC_MX_E4M3 one byte per element; MSC_MX_E2M1 two elements per byte, the even channel in the low nibble.  The last block of a row is
  *            zero-filled up to MSC_MX_BLOCK, so a row takes nb*32 (nb*16) bytes, nb = ceil(C/32); codes_ld bytes from row to row, a multiple of 16,
  *            base 16-byte aligned.
- *   scales : one byte per block, nb bytes per row, scales_ld bytes from row to row.  Byte e stands for 2^(e-127), 255 for NaN.
+ *   scales : one byte per block, nb bytes per row, scales_ld bytes from row to row.  Byte e (1 .. 254) stands for 2^(e-127), 255 for NaN.
  *   value  : code * 2^(e-127).
  * Packing takes the smallest power of two under which no element passes the largest code (448 / 6) and rounds to the nearest code, ties to even
  * (an error of at most 2^-4 / 2^-2 of the value, or half the smallest code times the scale).  Elements whose code would stand for a value past the
@@ -531,7 +531,7 @@ int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream);
  *   dy = gamma*invstd*(dh - mean(dh) - xhat*mean(dh*xhat));  dres = dh (dres may be NULL; dres_acc: dres += dh)
  * relu 0: no mask; 2: [scale*y + shift > 0] from the stored y; 3: the byte mask msc_bn_apply wrote (relu_mask, mask_ld bytes per row) -- the
  * forward's own, which 2 can only approximate.  dy or dres may be dout itself (same ld): each element is read before it is written.
- * gamma NULL: ones; dgamma / dbeta NULL: not wanted.  ws: msc_mx_bn_bwd_workspace_bytes() bytes, 16-byte aligned. */
+ * gamma NULL: ones; dgamma / dbeta NULL: not wanted.  ws: msc_mx_bn_bwd_workspace_bytes() bytes (0 for few rows), 16-byte aligned. */
 typedef struct msc_mx_bn_bwd_desc {
     const void* dout;
     const uint8_t* y;

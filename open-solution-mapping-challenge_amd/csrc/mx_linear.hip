@@ -3,9 +3,11 @@
 // on v_mfma_scale_f32_16x16x128_f8f6f4: a lane feeds 32 consecutive k of one row (16 bytes of codes, one block) and that block's scale byte, so the
 // stored layout is the instruction's own and nothing is re-laid out.  Products of codes are exact, the sums fp32.
 //
-// Operand roles.  w is the instruction's A operand (rows of the result: n), x its B operand (columns: m): a lane then holds consecutive n of one m.  The
-// fragment rows are dealt out so that fragment f, row i is channel 16*(i >> 2) + 4*f + (i & 3) of a wave's 64: the four fragments of a lane make 16
-// consecutive channels, whose scale / shift / res / out move in 16-byte pieces, 128 bytes of a row per wave instruction.
+// Operand roles.  w is the instruction's A operand (rows of the result: n), x its B operand (columns: m): a lane then holds consecutive n of one m, and the
+// fragment rows are dealt out so that its fragments make two runs of eight channels, which move in 16-byte pieces.
+//
+// Three forms: up to 16 (64) rows, the weights streamed once by blocks of 16 channels; a few tiles' channels, x quantised by the tile kernel itself; else packing,
+// then tiles of 256 x 256 (fewer: 128 x 128, 64 x 64).
 #include <type_traits>
 
 #include "common.h"
@@ -23,212 +25,336 @@ struct LinArgs {
     const uint8_t* x; const uint8_t* xs; const uint8_t* w; const uint8_t* ws;
     const float* scale; const float* shift; const void* res; void* out;
     long x_ld, xs_ld, w_ld, ws_ld, res_ld, out_ld, M;
-    int K, N, nb, tiles_n, relu;         // nb: blocks of 32 along k
-    int xs_quick, ws_quick;              // the eight scales of a step are one aligned load
+    int K, N, nb, tiles_m, tiles_n, relu;         // nb: blocks of 32 along k
 };
 
 __device__ __forceinline__ i32x8 fp4_operand(uint4 v) { return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
 
-// CNT (a multiple of 8) consecutive channels from n: their scale / shift, and one row's results
-template <typename T, int CNT, bool VEC> struct Epilogue {
-    float sc[CNT], sh[CNT];
+// eight consecutive channels from n: their scale / shift; one row's residual, and its results.  Apart, because res may be out: a loop that loads and stores row by
+// row could not have the next row's load in flight
+template <typename T, bool VEC> struct Epilogue {
+    static constexpr int PIECES = sizeof(T) / 2;
+    struct Res { uint4 v[PIECES]; };
+    float sc[8], sh[8];
     int n, left;
     __device__ __forceinline__ Epilogue(const LinArgs& a, int n_) : n(n_), left(a.N - n_) {
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) {
+        for (int i = 0; i < 8; ++i) {
             sc[i] = a.scale && i < left ? a.scale[n + i] : 1.f;
             sh[i] = a.shift && i < left ? a.shift[n + i] : 0.f;
         }
     }
-    __device__ __forceinline__ void row(const LinArgs& a, long m, const float* v) const {
-        if (left <= 0) return;
+    __device__ __forceinline__ Res load(const LinArgs& a, long m, bool in) const {
+        Res r;
 #pragma unroll
-        for (int h = 0; h < CNT; h += 8) {
-            float r[8];
-            const T* rp = (const T*)a.res + m * a.res_ld + n + h;
-            if (!a.res) {
+        for (int k = 0; k < PIECES; ++k) r.v[k] = make_uint4(0, 0, 0, 0);
+        if (!a.res || left <= 0 || !in) return r;
+        const T* p = (const T*)a.res + m * a.res_ld + n;
+        if (VEC && left >= 8) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) r[i] = 0.f;
-            } else if (VEC && left >= h + 8) load8<T>(rp, r);
-            else load8_some<T>(rp, left - h, r);
+            for (int k = 0; k < PIECES; ++k) r.v[k] = reinterpret_cast<const uint4*>(p)[k];
+        } else {
+            float v[8];
+            load8_some<T>(p, left, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = fmaf(v[h + i], sc[h + i], sh[h + i]) + r[i];
-                r[i] = a.relu && y < 0.f ? 0.f : y;            // NaN stays NaN
-            }
-            T* o = (T*)a.out + m * a.out_ld + n + h;
-            if (VEC && left >= h + 8) store8<T>(o, r);
-            else store8_some<T>(o, left - h, r);
+            for (int k = 0; k < PIECES; ++k) r.v[k] = Vec16<T>::pack(v + k * Vec16<T>::N);
         }
+        return r;
+    }
+    __device__ __forceinline__ void store(const LinArgs& a, long m, bool in, const Res& res, const float* v) const {
+        if (left <= 0 || !in) return;
+        float r[8];
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) Vec16<T>::unpack(res.v[k], r + k * Vec16<T>::N);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = fmaf(v[i], sc[i], sh[i]) + r[i];
+            r[i] = a.relu && y < 0.f ? 0.f : y;                        // NaN stays NaN
+        }
+        T* o = (T*)a.out + m * a.out_ld + n;
+        if (VEC && left >= 8) store8<T>(o, r);
+        else store8_some<T>(o, left, r);
     }
 };
 
 // ------------------------------------------------------------------------------------------------ many rows
-// WM x WN waves, each FM x 4 fragments: a tile of 16*WM*FM rows by 64*WN channels per block.  A step is 256 k (eight blocks, 128 bytes of codes and eight scale
-// bytes) of every row, double-buffered in LDS: the codes by LDS-DMA, straight from the stored layout, the next step's requests going out before this step's
-// products.  16-byte unit u of LDS row r sits at u ^ ((r >> 1) & 7) (the DMA's source is permuted, its destination is linear): the 16 rows of a fragment
-// read fall into all the banks.  The scales go through registers and are dealt out as [wave row][lane group][fragment row][fragment] pairs of bytes, so
-// that a lane has those of all its fragments in one read; loading them per lane from memory (two byte loads a fragment and step, 16 rows of a wave each) took
-// several times as long as the products.
+// WM x WN waves, each FM x 4 fragments: a tile of 16*WM*FM rows by 64*WN channels at a time, a block takes several.  A step is 256 k (eight blocks: 128 bytes
+// of codes and eight of scales) of every row, filled into one half of LDS by LDS-DMA straight from the stored layout while the other is multiplied; the first step
+// of the next tile goes out before the last one of this tile, so that it lands during the products and the epilogue.  16-byte unit u of LDS row r sits at
+// u ^ ((r >> 1) & 7) (the DMA's source is permuted, its destination is linear) and lane group g takes the units g and g + 4: the 16 lanes that a 16-byte read
+// serves together (rows 0-3 and 12-15 of one group, 4-11 of the next) then fall into 16 different bank quads.  (Units 2g and 2g + 1 made them collide in
+// pairs: SQ_LDS_BANK_CONFLICT was 48 % of SQ_LDS_IDX_ACTIVE.)  Scales by the dword, too: byte loads per lane and fragment took several times the products'
+// time, a detour through registers a tenth of it.
 constexpr int UNITS = 8, ROWB = UNITS * 16;
+
+// 4 bytes per lane from buffer offset `voff` to LDS bytes [lds_wave_base, +256)
+__device__ __forceinline__ void dma4(u32x4_t srd, char* lds_wave_base, unsigned voff) {
+    const unsigned lds_addr = (unsigned)(size_t)(lds_ptr_t)lds_wave_base;
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(lds_addr), "v"(voff), "s"(srd)
+                 : "memory");
+}
+
+// w's LDS row 16 f + i of a wave's 64 is this channel of its 64: a lane's fragments 0, 1 and 2, 3 are eight consecutive channels each, 64 bytes of a 16-bit row
+// over the four lane groups
+__device__ __forceinline__ int lin_channel(int slot) { return (slot & ~63) + 32 * (slot >> 5 & 1) + 8 * ((slot & 15) >> 2) + 4 * (slot >> 4 & 1) + (slot & 3); }
+
+// one step's products of a wave: FM fragments of rows from LDS row wm * FM * 16, four of channels from LDS row TM + wn * 64
+template <int FM, int TM> __device__ __forceinline__ void lin_step(const LinArgs& a, int s, const char* st, int SCALES, int wm, int wn, int g, int pl, f32x4 (&acc)[FM][4]) {
+    constexpr int FN = 4;
+    int qx[2][FM], qw[2][FN];        // byte 0: the scale of unit g / g + 4
+    const char* pws = st + SCALES + (TM + wn * 64 + pl) * 8;
+    const char* pxs = st + SCALES + (wm * (FM * 16) + pl) * 8;
+    auto both = [&](const char* p, int& q0, int& q1) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        q0 = (int)(v.x >> 8 * g);
+        q1 = (int)(v.y >> 8 * g);
+    };
+#pragma unroll
+    for (int f = 0; f < FN; ++f) both(pws + f * 128, qw[0][f], qw[1][f]);
+#pragma unroll
+    for (int f = 0; f < FM; ++f) both(pxs + f * 128, qx[0][f], qx[1][f]);
+    if (s * UNITS + UNITS > a.nb) {  // past the last block the codes are zero: any scale but the NaN one
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool past = s * UNITS + 4 * h + g >= a.nb;
+#pragma unroll
+            for (int f = 0; f < FN; ++f) qw[h][f] = past ? 127 : qw[h][f];
+#pragma unroll
+            for (int f = 0; f < FM; ++f) qx[h][f] = past ? 127 : qx[h][f];
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint4 fx[FM], fw[FN];
+#pragma unroll
+        for (int f = 0; f < FN; ++f) {
+            const int r = wn * 64 + f * 16 + pl;
+            fw[f] = *reinterpret_cast<const uint4*>(st + (TM + r) * ROWB + ((g + 4 * h) ^ ((r >> 1) & 7)) * 16);
+        }
+#pragma unroll
+        for (int f = 0; f < FM; ++f) {
+            const int r = wm * (FM * 16) + f * 16 + pl;
+            fx[f] = *reinterpret_cast<const uint4*>(st + r * ROWB + ((g + 4 * h) ^ ((r >> 1) & 7)) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(fw[j]), fp4_operand(fx[i]), acc[i][j], 4, 4, 0, qw[h][j], 0, qx[h][i]);
+    }
+}
+
+// ... and their results.  Fragments 2h, 2h + 1 of a lane are channels 32 h + 8 g .. + 7 of the wave's 64, of row pl: stored as they are, an instruction would write 64
+// bytes of each of 16 rows.  Neighbours pl, pl ^ 1 swap halves first: the even lane takes channels 8 g of both rows, the odd lane channels 32 + 8 g, and an
+// instruction writes whole 128-byte lines of eight rows (131072 x 64 -> 256: 28.0 ->
+// 25.8 us)
+template <typename T, int FM, bool VEC>
+__device__ __forceinline__ void lin_write(const LinArgs& a, long m0, int last_m, int n0, int wm, int wn, int g, int pl, const f32x4 (&acc)[FM][4]) {
+    using E = Epilogue<T, VEC>;
+    const bool odd = pl & 1;
+    const E ep(a, n0 + wn * 64 + (odd ? 32 : 0) + 8 * g);
+    constexpr int ROWS = FM < 4 ? FM : 4;
+#pragma unroll
+    for (int i0 = 0; i0 < FM; i0 += ROWS) {
+        typename E::Res r0[ROWS], r1[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int m = wm * (FM * 16) + (i0 + k) * 16 + (pl & ~1);
+            r0[k] = ep.load(a, m0 + m, m <= last_m);
+            r1[k] = ep.load(a, m0 + m + 1, m + 1 <= last_m);
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int i = i0 + k, m = wm * (FM * 16) + i * 16 + (pl & ~1);
+            float v0[8], v1[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float lo = acc[i][c / 4][c % 4], hi = acc[i][2 + c / 4][c % 4];
+                const float got = __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(odd ? lo : hi), 0xB1, 0xF, 0xF, true));      // quad_perm [1,0,3,2]
+                v0[c] = odd ? got : lo;
+                v1[c] = odd ? hi : got;
+            }
+            ep.store(a, m0 + m, m <= last_m, r0[k], v0);
+            ep.store(a, m0 + m + 1, m + 1 <= last_m, r1[k], v1);
+        }
+    }
+}
 
 template <typename T, int WM, int WN, int FM, bool VEC>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(LinArgs a) {
-    constexpr int THREADS = WM * WN * 64, WAVES = WM * WN, FN = 4, TM = WM * FM * 16, TN = WN * 64;
-    constexpr int DX = TM / 8 / WAVES, DW = TN / 8 / WAVES;            // DMA instructions (8 rows each) per wave and step
-    constexpr int SCALES = (TM + TN) * ROWB, STAGE = SCALES + (TM + TN) * UNITS, NS = (TM + TN + THREADS - 1) / THREADS;
-    static_assert(TM / 8 % WAVES == 0 && TN / 8 % WAVES == 0, "every wave requests");
+    constexpr int WAVES = WM * WN, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN;
+    constexpr int DX = TM / 8 / WAVES, DW = TN / 8 / WAVES;            // DMA instructions (8 rows of codes each) per wave and step
+    constexpr int DSX = (TM / 32 + WAVES - 1) / WAVES, DSW = (TN / 32 + WAVES - 1) / WAVES;      // ... of scales (32 rows); a wave past the last repeats it
+    constexpr int SCALES = ROWS * ROWB, STAGE = SCALES + ROWS * 8;
+    static_assert(TM / 8 % WAVES == 0 && TN / 8 % WAVES == 0 && TM % 32 == 0, "every wave requests");
     static_assert(2 * STAGE <= 160 * 1024, "LDS");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wid / WN, wn = wid % WN, g = lane >> 4, pl = lane & 15;
-    const int tn = (int)(blockIdx.x % (unsigned)a.tiles_n);
-    const long m0 = (long)(blockIdx.x / (unsigned)a.tiles_n) * TM;
-    const int n0 = tn * TN;
     const int steps = (a.nb + UNITS - 1) / UNITS;
-    const int last_m = (int)min((long)TM, a.M - m0) - 1, last_n = min(TN, a.N - n0) - 1;      // rows past the end: the last one again, their results are dropped
+    // (The order of the tiles over the XCDs and the place in k where each starts were tried both ways: within 2 % of each other.)
+    const unsigned tiles = (unsigned)a.tiles_m * (unsigned)a.tiles_n;
 
-    // w's LDS row 16 f + i of a wave's 64 is channel 16*(i >> 2) + 4*f + (i & 3)
-    auto channel = [](int slot) { return (slot & ~63) + 16 * ((slot & 15) >> 2) + 4 * ((slot >> 4) & 3) + (slot & 3); };
-    const u32x4_t rx = make_srd(a.x + m0 * a.x_ld, (unsigned)(last_m * a.x_ld + a.nb * 16));
-    const u32x4_t rw = make_srd(a.w + (long)n0 * a.w_ld, (unsigned)(last_n * a.w_ld + a.nb * 16));
-    unsigned xo[DX], wo[DW];
-    int xu[DX], wu[DW];
-#pragma unroll
-    for (int i = 0; i < DX; ++i) {
-        const int r = (i * WAVES + wid) * 8 + (lane >> 3);
-        xu[i] = (lane & 7) ^ ((r >> 1) & 7);
-        xo[i] = (unsigned)min(r, last_m) * (unsigned)a.x_ld + xu[i] * 16;
-    }
-#pragma unroll
-    for (int i = 0; i < DW; ++i) {
-        const int r = (i * WAVES + wid) * 8 + (lane >> 3);
-        wu[i] = (lane & 7) ^ ((r >> 1) & 7);
-        wo[i] = (unsigned)min(channel(r), last_n) * (unsigned)a.w_ld + wu[i] * 16;
-    }
-    auto request = [&](int s, char* st) {                              // the codes of step s; blocks past the last one read as zeros
-#pragma unroll
-        for (int i = 0; i < DX; ++i) dma16(rx, st + (i * WAVES + wid) * 1024, s * UNITS + xu[i] < a.nb ? xo[i] + s * ROWB : OOB_OFF, 0);
-#pragma unroll
-        for (int i = 0; i < DW; ++i) dma16(rw, st + TM * ROWB + (i * WAVES + wid) * 1024, s * UNITS + wu[i] < a.nb ? wo[i] + s * ROWB : OOB_OFF, 0);
+    struct Place { long m0; int n0, last_m, last_n; };
+    auto place = [&](unsigned id) {
+        Place p;
+        p.m0 = (long)(id / (unsigned)a.tiles_n) * TM;
+        p.n0 = (int)(id % (unsigned)a.tiles_n) * TN;
+        p.last_m = (int)min((long)TM, a.M - p.m0) - 1;                 // rows past the end: the last one again, their results are dropped
+        p.last_n = min(TN, a.N - p.n0) - 1;
+        return p;
     };
-    // scales: thread t moves the eight of LDS rows t, t + THREADS (x's rows, then w's)
-    const uint8_t* sp[NS];
-    int so[NS], sf[NS];                  // LDS place for lane group 0; bytes from lane group to lane group
-    bool quick[NS];
+    u32x4_t rx, rw, rxs, rws;
+    unsigned xo[DX], wo[DW], xso[DSX], wso[DSW];
+    const int u = (lane & 7) ^ ((wid * 8 + (lane >> 3)) >> 1 & 7);     // of the lane's rows, 8 * WAVES apart: one key where WAVES is even
+    static_assert(WAVES % 2 == 0, "unit key");
+    auto aim = [&](const Place& p) {
+        rx = make_srd(a.x + p.m0 * a.x_ld, (unsigned)(p.last_m * a.x_ld + a.nb * 16));
+        rw = make_srd(a.w + (long)p.n0 * a.w_ld, (unsigned)(p.last_n * a.w_ld + a.nb * 16));
+        rxs = make_srd(a.xs + p.m0 * a.xs_ld, (unsigned)(p.last_m * a.xs_ld + (a.nb + 3) / 4 * 4));
+        rws = make_srd(a.ws + (long)p.n0 * a.ws_ld, (unsigned)(p.last_n * a.ws_ld + (a.nb + 3) / 4 * 4));
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int r = i * THREADS + tid;
-        if (r < TM) {
-            sp[i] = a.xs + (m0 + min(r, last_m)) * a.xs_ld;
-            so[i] = SCALES + ((r / (FM * 16) * 64 + r % 16) * FM + r % (FM * 16) / 16) * 2;
-            sf[i] = FM * 32;
-            quick[i] = a.xs_quick;
-        } else {
-            const int w = min(r - TM, TN - 1);
-            sp[i] = a.ws + (long)(n0 + min(channel(w), last_n)) * a.ws_ld;
-            so[i] = SCALES + TM * UNITS + ((w / 64 * 64 + w % 16) * FN + w % 64 / 16) * 2;
-            sf[i] = FN * 32;
-            quick[i] = a.ws_quick;
+        for (int i = 0; i < DX; ++i) xo[i] = (unsigned)min((i * WAVES + wid) * 8 + (lane >> 3), p.last_m) * (unsigned)a.x_ld + u * 16;
+#pragma unroll
+        for (int i = 0; i < DW; ++i) wo[i] = (unsigned)min(lin_channel((i * WAVES + wid) * 8 + (lane >> 3)), p.last_n) * (unsigned)a.w_ld + u * 16;
+#pragma unroll
+        for (int i = 0; i < DSX; ++i) xso[i] = (unsigned)min(min(i * WAVES + wid, TM / 32 - 1) * 32 + (lane >> 1), p.last_m) * (unsigned)a.xs_ld + (lane & 1) * 4;
+#pragma unroll
+        for (int i = 0; i < DSW; ++i) wso[i] = (unsigned)min(lin_channel(min(i * WAVES + wid, TN / 32 - 1) * 32 + (lane >> 1)), p.last_n) * (unsigned)a.ws_ld + (lane & 1) * 4;
+    };
+    auto request = [&](int s, char* st) {                              // blocks past the last one read as zeros
+        const bool live = s * UNITS + u < a.nb, live_s = s * UNITS + (lane & 1) * 4 < a.nb;
+#pragma unroll
+        for (int i = 0; i < DX; ++i) dma16(rx, st + (i * WAVES + wid) * 1024, live ? xo[i] + s * ROWB : OOB_OFF, 0);
+#pragma unroll
+        for (int i = 0; i < DW; ++i) dma16(rw, st + TM * ROWB + (i * WAVES + wid) * 1024, live ? wo[i] + s * ROWB : OOB_OFF, 0);
+#pragma unroll
+        for (int i = 0; i < DSX; ++i) dma4(rxs, st + SCALES + min(i * WAVES + wid, TM / 32 - 1) * 256, live_s ? xso[i] + s * UNITS : OOB_OFF);
+#pragma unroll
+        for (int i = 0; i < DSW; ++i) dma4(rws, st + SCALES + TM * 8 + min(i * WAVES + wid, TN / 32 - 1) * 256, live_s ? wso[i] + s * UNITS : OOB_OFF);
+    };
+
+    f32x4 acc[FM][FN];
+    Place here = place(blockIdx.x);
+    aim(here);
+    int half = 0;
+    request(0, smem);
+    for (unsigned id = blockIdx.x; id < tiles; id += gridDim.x) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const Place next = place(min(id + gridDim.x, tiles - 1));
+        for (int s = 0; s < steps; ++s) {
+            wait_vmcnt<0>();                                           // this wave's requests of this step have landed ...
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // ... its reads of the last one are done ...
+            raw_barrier();                                             // ... and so for the others: the other half is free
+            if (s + 1 < steps) {
+                request(s + 1, smem + (half ^ 1) * STAGE);
+            } else if (id + gridDim.x < tiles) {
+                aim(next);
+                request(0, smem + (half ^ 1) * STAGE);
+            }
+            lin_step<FM, TM>(a, s, smem + half * STAGE, SCALES, wm, wn, g, pl, acc);
+            half ^= 1;
         }
+        lin_write<T, FM, VEC>(a, here.m0, here.last_m, here.n0, wm, wn, g, pl, acc);
+        here = next;
     }
-    uint2 rs[NS];
-    auto fetch_scales = [&](int s) {
+}
+
+// ------------------------------------------------------------------------------------------------ few channels
+// The same tile, with x quantised on the way into LDS instead of by a launch of its own: for weights of a few tiles' channels, where every row of x is then
+// quantised once or a few times.  x comes through registers (a quad of lanes a block, as in packing), w by LDS-DMA.  WM x WN = 4 waves, FM fragments of rows each.
+template <typename T, int WM, int WN, int FM, bool VEC>
+__global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xin, long xin_ld, int xvec) {
+    constexpr int WAVES = 4, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN, DW = TN / 8 / WAVES, DSW = (TN / 32 + WAVES - 1) / WAVES;
+    constexpr int SCALES = ROWS * ROWB, STAGE = SCALES + ROWS * 8, CHUNKS = TM * UNITS * 4 / 256;
+    static_assert(WM * WN == WAVES && 2 * STAGE <= 80 * 1024, "two blocks per CU");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wid / WN, wn = wid % WN, g = lane >> 4, pl = lane & 15;
+    const int steps = (a.nb + UNITS - 1) / UNITS;
+    const long m0 = (long)(blockIdx.x / (unsigned)a.tiles_n) * TM;
+    const int n0 = (int)(blockIdx.x % (unsigned)a.tiles_n) * TN;
+    const int last_m = (int)min((long)TM, a.M - m0) - 1, last_n = min(TN, a.N - n0) - 1;
+    const u32x4_t rw = make_srd(a.w + (long)n0 * a.w_ld, (unsigned)(last_n * a.w_ld + a.nb * 16));
+    const u32x4_t rws = make_srd(a.ws + (long)n0 * a.ws_ld, (unsigned)(last_n * a.ws_ld + (a.nb + 3) / 4 * 4));
+    const int u = (lane & 7) ^ ((wid * 8 + (lane >> 3)) >> 1 & 7);
+    unsigned wo[DW], wso[DSW];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if (i * THREADS + tid >= TM + TN) continue;
-            if (quick[i]) {
-                rs[i] = *reinterpret_cast<const uint2*>(sp[i] + s * UNITS);
-            } else {                     // past the last block the codes are zero: any scale but the NaN one
-                unsigned b[UNITS];
+    for (int i = 0; i < DW; ++i) wo[i] = (unsigned)min(lin_channel((i * WAVES + wid) * 8 + (lane >> 3)), last_n) * (unsigned)a.w_ld + u * 16;
 #pragma unroll
-                for (int k = 0; k < UNITS; ++k) b[k] = s * UNITS + k < a.nb ? sp[i][s * UNITS + k] : 127u;
-                rs[i] = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+    for (int i = 0; i < DSW; ++i) wso[i] = (unsigned)min(lin_channel(min(i * WAVES + wid, TN / 32 - 1) * 32 + (lane >> 1)), last_n) * (unsigned)a.ws_ld + (lane & 1) * 4;
+    auto request = [&](int s, char* st) {
+        const bool live = s * UNITS + u < a.nb, live_s = s * UNITS + (lane & 1) * 4 < a.nb;
+#pragma unroll
+        for (int i = 0; i < DW; ++i) dma16(rw, st + TM * ROWB + (i * WAVES + wid) * 1024, live ? wo[i] + s * ROWB : OOB_OFF, 0);
+#pragma unroll
+        for (int i = 0; i < DSW; ++i) dma4(rws, st + SCALES + TM * 8 + min(i * WAVES + wid, TN / 32 - 1) * 256, live_s ? wso[i] + s * UNITS : OOB_OFF);
+    };
+    // chunk i of thread t: eight channels, number t % 32 of a step, of row t / 32 + 8 i
+    const int xr = tid >> 5, xc = tid & 31;
+    constexpr int PIECES = sizeof(T) / 2;                              // 16-byte pieces of a chunk, kept as they were loaded
+    uint4 xv[CHUNKS][PIECES];
+    auto fetch = [&](int s) {
+        const int k = s * (UNITS * BLOCK) + xc * 8, left = a.K - k;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const T* p = xin + (m0 + min(xr + 8 * i, last_m)) * xin_ld + k;
+            if (xvec && left >= 8) {
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) xv[i][k] = reinterpret_cast<const uint4*>(p)[k];
+            } else {
+                float v[8];
+                load8_some<T>(p, left, v);
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) xv[i][k] = Vec16<T>::pack(v + k * Vec16<T>::N);
             }
         }
     };
-    auto put_scales = [&](char* st) {
+    auto put = [&](char* st) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if (i * THREADS + tid >= TM + TN) continue;
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int r = xr + 8 * i, b = xc >> 2;
+            float v[8], q[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) *reinterpret_cast<uint16_t*>(st + so[i] + k * sf[i]) = (uint16_t)((k < 2 ? rs[i].x : rs[i].y) >> (k & 1) * 16);
+            for (int k = 0; k < PIECES; ++k) Vec16<T>::unpack(xv[i][k], v + k * Vec16<T>::N);
+            const unsigned e = block_scale<E2M1, T>(v, q);
+            *reinterpret_cast<unsigned*>(st + r * ROWB + (b ^ ((r >> 1) & 7)) * 16 + (xc & 3) * 4) = encode8_e2m1(q);
+            if ((xc & 3) == 0) st[SCALES + r * 8 + b] = (char)e;
         }
     };
-
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto compute = [&](const char* st) {
-        int qx[FM / 2], qw[FN / 2];      // two fragments to a register, two bytes each
-        const char* px = st + SCALES + ((wm * 4 + g) * 16 + pl) * FM * 2;
-        const char* pw = st + SCALES + TM * UNITS + ((wn * 4 + g) * 16 + pl) * FN * 2;
-#pragma unroll
-        for (int k = 0; k < FM / 2; ++k) qx[k] = reinterpret_cast<const int*>(px)[k];
-#pragma unroll
-        for (int k = 0; k < FN / 2; ++k) qw[k] = reinterpret_cast<const int*>(pw)[k];
-        auto half = [&](auto hh) {
-            constexpr int H = decltype(hh)::value;
-            uint4 fx[FM], fw[FN];
-#pragma unroll
-            for (int f = 0; f < FN; ++f) {
-                const int r = wn * 64 + f * 16 + pl;
-                fw[f] = *reinterpret_cast<const uint4*>(st + (TM + r) * ROWB + ((2 * g + H) ^ ((r >> 1) & 7)) * 16);
-            }
-#pragma unroll
-            for (int f = 0; f < FM; ++f) {
-                const int r = wm * (FM * 16) + f * 16 + pl;
-                fx[f] = *reinterpret_cast<const uint4*>(st + r * ROWB + ((2 * g + H) ^ ((r >> 1) & 7)) * 16);
-            }
-            // the scale's byte is an immediate: even and odd fragments apart
-            auto one = [&](auto ii, auto jj, int i, int j) {
-                constexpr int SX = decltype(ii)::value * 2 + H, SW = decltype(jj)::value * 2 + H;
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(fw[j]), fp4_operand(fx[i]), acc[i][j], 4, 4, SW, qw[j / 2], SX, qx[i / 2]);
-            };
-#pragma unroll
-            for (int i = 0; i < FM; i += 2)
-#pragma unroll
-                for (int j = 0; j < FN; j += 2) {
-                    one(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, i, j);
-                    one(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, i, j + 1);
-                    one(std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{}, i + 1, j);
-                    one(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, i + 1, j + 1);
-                }
-        };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
-    };
-
-    fetch_scales(0);
+    fetch(0);
     request(0, smem);
-    put_scales(smem);
-    wait_vmcnt<0>();
-    __syncthreads();
+    put(smem);
     for (int s = 0; s < steps; ++s) {
-        char* next = smem + ((s + 1) & 1) * STAGE;                     // last read two barriers ago
+        char* const now = smem + (s & 1) * STAGE;
+        char* const next = smem + ((s + 1) & 1) * STAGE;
+        wait_vmcnt<0>();                                               // the requests of step s, which the compiler does not see
+        __syncthreads();                                               // ... and everyone's, x's codes among them; the other half is free
         if (s + 1 < steps) {
-            fetch_scales(s + 1);
+            fetch(s + 1);
             request(s + 1, next);
         }
-        compute(smem + (s & 1) * STAGE);
-        if (s + 1 < steps) put_scales(next);
-        wait_vmcnt<0>();                 // the requests, which the compiler does not see
-        __syncthreads();
+        lin_step<FM, TM>(a, s, now, SCALES, wm, wn, g, pl, acc);
+        if (s + 1 < steps) put(next);
     }
-    // fragment f, result row 4 g + r: channel 16 g + 4 f + r of the wave's 64
-    const Epilogue<T, 4 * FN, VEC> ep(a, n0 + wn * 64 + 16 * g);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int m = wm * (FM * 16) + i * 16 + pl;
-        float v[4 * FN];
-#pragma unroll
-        for (int f = 0; f < FN; ++f)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[4 * f + r] = acc[i][f][r];
-        if (m <= last_m) ep.row(a, m0 + m, v);
-    }
+    lin_write<T, FM, VEC>(a, m0, last_m, n0, wm, wn, g, pl, acc);
+}
+
+// scales in rows a multiple of four bytes apart, for the kernel above
+__global__ __launch_bounds__(256) void mx_scale_rows_kernel(const uint8_t* __restrict__ in, long in_ld, uint8_t* __restrict__ out, long out_ld, long rows, int nb) {
+    for (long row = blockIdx.x * 4l + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4l)
+        for (int b = threadIdx.x & 63; b < nb; b += 64) out[row * out_ld + b] = in[row * in_ld + b];
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -330,17 +456,28 @@ template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREA
 
 constexpr int FUSED_ROWS = 16, FEW_ROWS = 64;
 constexpr int64_t FUSED_LDS = 64 * 1024;
+// x quantised by the tile kernel itself (mx_fused_kernel): for weights of at most two waves' channels, and where 512 blocks of 16 (32) x 256 cover the result and the
+// reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 11.7 : 17.5; 131072 x 256 -> 64 24 : 44; 32768 x 512 -> 128 15 : 21;
+// 2048 x 512 -> 2048 12.1 : 14.1; but 8192 x 1024 -> 1024 31 : 24, 1024 x 4096 -> 1024 28 : 22, 8192 x 4096 -> 512 48 : 44
+constexpr int FUSED_CHANNELS = 128, FUSED_BLOCKS = 512, FUSED_K = 1024;
 
-struct LinPlan { int64_t nb, xc_ld, codes, scales; bool pack, fused, few; };
+struct LinPlan { int64_t nb, xc_ld, s_ld, codes, scales, w_scales, bytes; bool pack, fused, few, tile; int tile_rows; };      // fused: few rows, tile: few channels -- x is quantised by the product's own launch
+bool dword_rows(const void* s, int64_t ld) { return ((uintptr_t)s & 3) == 0 && ld % 4 == 0; }
 LinPlan lin_plan(const msc_mx_linear_desc* d) {
     LinPlan p;
     p.nb = ((int64_t)d->K + BLOCK - 1) / BLOCK;
     p.fused = d->x && d->M <= FUSED_ROWS && few_lds(d->M, p.nb) <= FUSED_LDS;
     p.few = d->M <= FEW_ROWS;
-    p.pack = d->x && !p.fused;
+    const int64_t tiles = (d->M + 15) / 16 * ((d->N + 255) / 256);
+    p.tile_rows = tiles <= FUSED_BLOCKS ? 1 : 2;                // fragments of 16
+    p.tile = d->x && !p.few && (d->N <= FUSED_CHANNELS || (tiles <= 2 * FUSED_BLOCKS && d->K <= FUSED_K));
+    p.pack = d->x && !p.fused && !p.tile;
     p.xc_ld = p.nb * E2M1::BYTES;
+    p.s_ld = (p.nb + 3) / 4 * 4;                               // rows of scales start on dwords
     p.codes = p.pack ? d->M * p.xc_ld : 0;                     // a multiple of 16
-    p.scales = p.pack ? (d->M * p.nb + 15) / 16 * 16 : 0;
+    p.scales = p.pack || !(p.few || p.tile || dword_rows(d->x_scales, d->xs_ld)) ? (d->M * p.s_ld + 15) / 16 * 16 : 0;
+    p.w_scales = p.few || dword_rows(d->w_scales, d->s_ld) ? 0 : (d->N * p.s_ld + 15) / 16 * 16;
+    p.bytes = p.codes + p.scales + p.w_scales;
     return p;
 }
 
@@ -353,18 +490,35 @@ int lin_check(const msc_mx_linear_desc* d) {
 }
 
 template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, bool vec, hipStream_t st) {
-    constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS);
+    constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS), RESIDENT = 256 * (LDS > 80 * 1024 ? 1 : LDS > 40 * 1024 ? 2 : 4);
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
-    const int64_t blocks = (a.M + TM - 1) / TM * b.tiles_n;
-    if (blocks >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^31 tiles or more");
-    if (TM * a.x_ld >= 1ll << 31 || TN * a.w_ld >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
+    const int64_t tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * b.tiles_n;
+    b.tiles_m = (int)tiles_m;
+    if (tiles >= 1ll << 30) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^30 tiles or more");
+    if (TM * a.x_ld >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TM * a.xs_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
     auto k = vec ? mx_gemm_kernel<T, WM, WN, FM, true> : mx_gemm_kernel<T, WM, WN, FM, false>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return msc_fail(MSC_ERR_HIP, "msc_mx_linear: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(WM * WN * 64), LDS, st, b);
+    hipLaunchKernelGGL(k, dim3((unsigned)(tiles < RESIDENT ? tiles : RESIDENT)), dim3(WM * WN * 64), LDS, st, b);
+    return MSC_OK;
+}
+template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs& a, const msc_mx_linear_desc* d, bool vec, hipStream_t st) {
+    constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS);
+    LinArgs b = a;
+    b.tiles_n = (a.N + TN - 1) / TN;
+    const int64_t tiles = (a.M + TM - 1) / TM * b.tiles_n;
+    if (tiles >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^31 tiles or more, or a tile's rows span 2 GiB");
+    auto k = vec ? mx_fused_kernel<T, WM, WN, FM, true> : mx_fused_kernel<T, WM, WN, FM, false>;
+    if (LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return msc_fail(MSC_ERR_HIP, "msc_mx_linear: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), LDS, st, b, (const T*)d->x, (long)d->x_ld, (int)vec_ok(d->x, d->x_ld, d->dtype));
     return MSC_OK;
 }
 template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const msc_mx_linear_desc* d, bool vec, hipStream_t st) {
@@ -382,6 +536,12 @@ template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const 
         return MSC_OK;
     }
     auto tiles = [&](int tm, int tn) { return (a.M + tm - 1) / tm * ((a.N + tn - 1) / tn); };
+    if (p.tile) {
+        if (a.N <= 64) return lin_launch_fused<T, 4, 1, 1>(a, d, vec, st);
+        if (a.N <= 128) return lin_launch_fused<T, 2, 2, 2>(a, d, vec, st);
+        if (p.tile_rows == 1) return lin_launch_fused<T, 1, 4, 1>(a, d, vec, st);
+        return lin_launch_fused<T, 1, 4, 2>(a, d, vec, st);
+    }
     if (tiles(256, 256) >= 256) return lin_launch<T, 2, 4, 8>(a, vec, st);
     if (tiles(128, 128) >= 256) return lin_launch<T, 2, 2, 4>(a, vec, st);
     return lin_launch<T, 2, 1, 2>(a, vec, st);
@@ -392,7 +552,7 @@ template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const 
 extern "C" int64_t msc_mx_linear_workspace_bytes(const msc_mx_linear_desc* d) {
     if (lin_check(d)) return -1;
     const LinPlan p = lin_plan(d);
-    return p.codes + p.scales;
+    return p.bytes;
 }
 
 extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
@@ -407,25 +567,29 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_linear: w needs 16-byte aligned rows of whole E2M1 blocks and one scale byte per block");
     if (d->x && (d->x_ld < d->K || (uintptr_t)d->x % es))
         return msc_fail(MSC_ERR_ARG, "msc_mx_linear: x misaligned or row pitch %lld below %d channels", (long long)d->x_ld, d->K);
+    if (!d->x && !packed_ok(d->x_codes, d->xc_ld, d->x_scales, d->xs_ld, d->K, E2M1::BYTES))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_linear: x (or its codes: 16-byte aligned rows of whole E2M1 blocks, and scales) missing");
+    if (p.bytes && (!d->ws || (uintptr_t)d->ws & 15)) return msc_fail(MSC_ERR_ARG, "msc_mx_linear: workspace missing or not 16-byte aligned");
     LinArgs a;
-    a.x = a.xs = nullptr;
-    a.x_ld = a.xs_ld = 0;
+    uint8_t* codes = (uint8_t*)d->ws;
+    uint8_t* scales = codes + p.codes;
+    a.x = d->x_codes; a.x_ld = d->xc_ld; a.xs = d->x_scales; a.xs_ld = d->xs_ld;
+    a.ws = d->w_scales; a.ws_ld = d->s_ld;
     if (p.pack) {
-        if (!d->ws || (uintptr_t)d->ws & 15) return msc_fail(MSC_ERR_ARG, "msc_mx_linear: workspace missing or not 16-byte aligned");
-        uint8_t* codes = (uint8_t*)d->ws;
-        a.x = codes; a.x_ld = p.xc_ld; a.xs = codes + p.codes; a.xs_ld = p.nb;
-        rc = msc_mx_pack(d->x, d->x_ld, d->dtype, codes, p.xc_ld, codes + p.codes, p.nb, MSC_MX_E2M1, d->M, d->K, stream);
+        a.x = codes; a.x_ld = p.xc_ld; a.xs = scales; a.xs_ld = p.s_ld;
+        rc = msc_mx_pack(d->x, d->x_ld, d->dtype, codes, p.xc_ld, scales, p.s_ld, MSC_MX_E2M1, d->M, d->K, stream);
         if (rc) return rc;
-    } else if (!d->x) {
-        if (!packed_ok(d->x_codes, d->xc_ld, d->x_scales, d->xs_ld, d->K, E2M1::BYTES))
-            return msc_fail(MSC_ERR_ARG, "msc_mx_linear: x (or its codes: 16-byte aligned rows of whole E2M1 blocks, and scales) missing");
-        a.x = d->x_codes; a.x_ld = d->xc_ld; a.xs = d->x_scales; a.xs_ld = d->xs_ld;
     }
-    a.w = d->w; a.w_ld = d->w_ld; a.ws = d->w_scales; a.ws_ld = d->s_ld;
+    auto aligned_rows = [&](const uint8_t*& s, long& ld, int64_t rows, uint8_t* to) {
+        if (p.few || dword_rows(s, ld)) return;
+        hipLaunchKernelGGL(mx_scale_rows_kernel, dim3((unsigned)(rows < 4096 ? (rows + 3) / 4 : 1024)), dim3(256), 0, (hipStream_t)stream, s, ld, to, (long)p.s_ld, (long)rows, (int)p.nb);
+        s = to; ld = p.s_ld;
+    };
+    if (!p.tile) aligned_rows(a.xs, a.xs_ld, d->M, scales);
+    aligned_rows(a.ws, a.ws_ld, d->N, scales + p.scales);
+    a.w = d->w; a.w_ld = d->w_ld;
     a.scale = d->scale; a.shift = d->shift; a.res = d->res; a.out = d->out;
-    a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_n = 0;
-    auto quick = [&](const uint8_t* s, long ld) { return ((uintptr_t)s & 7) == 0 && ld % 8 == 0 && p.nb % UNITS == 0; };
-    a.xs_quick = quick(a.xs, a.xs_ld); a.ws_quick = quick(a.ws, a.ws_ld);
+    a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_m = a.tiles_n = 0;
     const bool vec = vec_ok(d->out, d->out_ld, d->dtype) && (!d->res || vec_ok(d->res, d->res_ld, d->dtype));
     hipStream_t st = (hipStream_t)stream;
     rc = d->dtype == MSC_F32 ? lin_by_tile<float>(a, p, d, vec, st) : d->dtype == MSC_BF16 ? lin_by_tile<bf16_t>(a, p, d, vec, st) : lin_by_tile<f16_t>(a, p, d, vec, st);

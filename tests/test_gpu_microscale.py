@@ -222,7 +222,8 @@ def bn_check(got, dout, y, gamma, mean, invstd, mask, dtype, residual):
 
 @pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
 @pytest.mark.parametrize('relu', ['none', 'bytes', 'coefficients'])
-@pytest.mark.parametrize('rows,c,residual', [(1, 1, False), (2, 7, True), (33, 40, True), (77, 75, False), (300, 256, True), (65, 300, False), (1000, 8, True)])
+@pytest.mark.parametrize('rows,c,residual', [(1, 1, False), (2, 7, True), (33, 40, True), (77, 75, False), (300, 256, True), (65, 300, False), (1000, 8, True), (2048, 24, True),
+                                             (2049, 40, True), (3000, 19, False)])
 def test_batchnorm_backward(rows, c, residual, relu, dtype):
     from mapping_challenge_amd import microscale as mx
     saved, y, mean, invstd, gamma, dout, mask, kw = bn_case(rows, c, dtype, rows + c, relu, residual)
@@ -232,8 +233,12 @@ def test_batchnorm_backward(rows, c, residual, relu, dtype):
 
 
 def test_batchnorm_backward_in_place_slices_and_repeats():
+    for rows, c in ((500, 96), (2500, 96)):                                # one launch, and three
+        check_batchnorm_in_place(rows, c)
+
+
+def check_batchnorm_in_place(rows, c):
     from mapping_challenge_amd import microscale as mx
-    rows, c = 500, 96
     saved, y, mean, invstd, gamma, dout, mask, kw = bn_case(rows, c, 'bf16', 31, 'bytes', True)
     cu = [torch.from_numpy(v).cuda() for v in (gamma, mean, invstd)]
     ref = mx.batchnorm_backward(dout.cuda(), saved, *cu, residual=True, **kw)
@@ -253,10 +258,10 @@ def test_batchnorm_backward_in_place_slices_and_repeats():
     assert torch.equal(none[0], ones[0])
 
 
-def test_batchnorm_backward_accumulates():
+@pytest.mark.parametrize('rows,c', [(200, 40), (2100, 40)])
+def test_batchnorm_backward_accumulates(rows, c):
     """dgamma / dbeta and dres added to what is there (the C entry's flags); a masked-out infinity or NaN in dout reaches nothing"""
     from mapping_challenge_amd import _lib, microscale as mx
-    rows, c = 200, 40
     saved, y, mean, invstd, gamma, dout, mask, kw = bn_case(rows, c, 'fp32', 41, 'bytes', True)
     cu = [torch.from_numpy(v).cuda() for v in (gamma, mean, invstd)]
     at = np.argwhere(~mask)

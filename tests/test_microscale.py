@@ -100,7 +100,7 @@ def test_batchnorm_refusals_and_workspace():
         refused(run(**bad), 'shape')
         assert lib.msc_mx_bn_bwd_workspace_bytes(bad.get('rows', 1), bad.get('C', 1)) == 0
     for bad in ('dout', 'dy', 'mean', 'invstd', 'ws'):
-        refused(run(**{bad: None}), 'null')
+        refused(run(rows=5000, **{bad: None}), 'null')
     refused(run(relu=1), 'relu')
     refused(run(relu=2), 'scale')
     refused(run(relu=3), 'mask')
@@ -114,7 +114,7 @@ def test_batchnorm_refusals_and_workspace():
     refused(run(dout=A16 + 1), 'aligned')
     refused(run(dres=2 * A16, dres_ld=64), 'different')                    # dy and dres in one buffer
     refused(run(dy=A16, dy_ld=80), 'pitch')                                # in place at another pitch
-    assert lib.msc_mx_bn_bwd_workspace_bytes(131072, 256) >= 256 * 32
+    assert lib.msc_mx_bn_bwd_workspace_bytes(131072, 256) >= 256 * 32 and lib.msc_mx_bn_bwd_workspace_bytes(100, 256) == 0      # few rows: one launch
 
 
 def linear_desc(**kw):
@@ -143,7 +143,7 @@ def test_linear_refusals_and_workspace():
     refused(run(x=None), 'x (or its codes')
     refused(run(x=None, x_codes=A16, x_scales=A16, xc_ld=16, xs_ld=2), 'x (or its codes')
     assert run(M=0) == 0
-    many = dict(M=1000, K=256, x_ld=256, w_ld=128, s_ld=8)
+    many = dict(M=1000, K=256, N=3000, x_ld=256, w_ld=128, s_ld=8, out_ld=3000)
     assert lib.msc_mx_linear_workspace_bytes(C.byref(linear_desc(**many))) >= 1000 * (128 + 8)
     refused(run(ws=None, **many), 'workspace')
     refused(run(ws=A16 + 4, **many), 'workspace')
