@@ -93,6 +93,10 @@ class BasePyTorchUNet(BaseTransformer):
         self.set_model()
         if (training_config or {}).get('deterministic') is not None:      # fixed-order gradient sums (UNetResNet.deterministic); default: MSC_DETERMINISTIC
             self.model.deterministic = bool(training_config['deterministic'])
+        if (training_config or {}).get('activation_checkpoint') is not None:      # 8-bit activation checkpoints (UNetResNet.activation_checkpoint)
+            if training_config['activation_checkpoint'] != 'e4m3':
+                raise ValueError("training_config['activation_checkpoint'] must be 'e4m3', got %r" % (training_config['activation_checkpoint'],))
+            self.model.activation_checkpoint = 'e4m3'
         opt = dict(architecture_config.get('optimizer_params', {}))
         reg = architecture_config.get('regularizer_params', {})
         wd = reg.get('weight_decay_conv2d', 0.0) if reg.get('regularize', False) else 0.0   # src/models.py:287-292

@@ -293,11 +293,18 @@ class UNetResNet(nn.Module):
     this mode: the BatchNorm / bias sums (per-XCD slots of float64 added in arrival order -- fp32 partials summed in double, so the
     result can differ between runs only when a rounding of the DOUBLE sum falls differently, which the repeat test has not seen but the
     arithmetic does not exclude); it needs MSC_WGRAD_GROUP > 1 and raises otherwise.
+    activation_checkpoint 'e4m3' (read when a training program is built): the encoder keeps what its backward needs of the forward -- every convolution's input
+    and every BatchNorm's input -- in 8 bits (microscaled E4M3, mapping_challenge_amd.microscale) and the ReLU masks as bits; the 16-bit activations and the
+    gradients that flow between two blocks live in a few buffers per shape.  The forward is unchanged; weight gradients and the BatchNorm backward see inputs
+    rounded to 3 mantissa bits.  The stem and the decoder stay as they are.
     """
 
     def __init__(self, encoder_depth, num_classes, num_filters=32, dropout_2d=0.2, pretrained=False,
-                 is_deconv=False, compute_dtype='bf16', autotune=None, deterministic=None):
+                 is_deconv=False, compute_dtype='bf16', autotune=None, deterministic=None, activation_checkpoint=None):
         super().__init__()
+        if activation_checkpoint not in (None, 'e4m3'):
+            raise ValueError("activation_checkpoint must be None or 'e4m3', got %r" % (activation_checkpoint,))
+        self.activation_checkpoint = activation_checkpoint
         self.deterministic = (_os_env.environ.get('MSC_DETERMINISTIC', '0') == '1') if deterministic is None else bool(deterministic)
         if encoder_depth not in _ENC:
             raise NotImplementedError('only 34, 101, 152 version of Resnet are implemented')
@@ -513,7 +520,7 @@ class UNetResNet(nn.Module):
 
     # ------------------------------------------------------------------ program construction
     def _program(self, N, H, W, training, device):
-        key = (N, H, W, training, self.compute_dtype)
+        key = (N, H, W, training, self.compute_dtype) + ((self.activation_checkpoint,) if training and self.activation_checkpoint else ())
         prog = self._programs.get(key)
         if prog is None:
             _quiesce(device)
@@ -741,6 +748,11 @@ class _Builder:
         self.bias_items = []          # (slots address, slot channel count, bias parameter, channels) awaiting flush_bias_slots
         self.fuse_bneck = _os_env.environ.get('MSC_FUSE_BNECK', '1') != '0'
         self.split_k = _os_env.environ.get('MSC_SPLIT_K', '1') != '0'
+        # 8-bit activation checkpoints of the encoder (UNetResNet.activation_checkpoint): `pool` holds the buffers that many layers use in turn
+        self.ckpt = bool(training and getattr(net, 'activation_checkpoint', None))
+        self.pool, self.transient, self.packs, self.mx_descs = {}, {}, {}, []
+        if self.ckpt:
+            self.bn_on_load = False
 
     # ---- memory
     def buf(self, H, W, C, dtype=None):
@@ -757,6 +769,49 @@ class _Builder:
 
     def act(self, H, W, C):
         return Act(self.buf(H, W, C))
+
+    def shared(self, key, H, W, C):
+        """an activation in memory that every request for `key` uses in turn: a tensor of its own (the bookkeeping goes by tensor), the same addresses.  Launches are
+        stream-ordered; what the backward needs of it is packed before the next layer writes.  'y': a raw convolution output, in the backward its gradient; 'm': an
+        activation inside a block, read by the next convolution only; 'o0' / 'o1': the outputs of a block and of the one before it, or of its downsample
+        branch.  Nothing of these is read again in the backward, so the gradients of 'm', 'o0', 'o1' take the same memory"""
+        n = self.N * H * W * C
+        base = self.pool.get(key)
+        if base is None or base.numel() < n:
+            base = self.pool[key] = self.buf(H, W, C)
+        t = base.view(-1)[:n].view(self.N, H, W, C)
+        self.prog.keep.append(t)
+        self.transient[id(t)] = key
+        return Act(t)
+
+    def block_act(self, key, H, W, C):
+        return self.shared(key, H, W, C) if self.ckpt else self.act(H, W, C)
+
+    def packed(self, a):
+        """the E4M3 checkpoint of activation `a` as (codes, scales), packed by the next forward launch if it is not yet"""
+        key = (id(a.buf), a.c0, a.C)
+        if key not in self.packs:
+            nb = (a.C + _lib.MX_BLOCK - 1) // _lib.MX_BLOCK
+            codes = torch.empty((self.N, a.H, a.W, nb * _lib.MX_BLOCK), dtype=torch.uint8, device=self.dev)
+            scales = torch.empty((self.N, a.H, a.W, nb), dtype=torch.uint8, device=self.dev)
+            self.prog.bytes += codes.numel() + scales.numel()
+            self.prog.keep += [codes, scales]
+            self.emit(self.prog.fwd, self.lib.msc_mx_pack, a.ptr, a.ld, self.dt, codes.data_ptr(), nb * _lib.MX_BLOCK, scales.data_ptr(), nb, _lib.MX_E4M3, a.pixels, a.C)
+            self.packs[key] = (codes, scales)
+        return self.packs[key]
+
+    def mx_ws(self, d, nbytes):
+        """descriptor `d` of a msc_mx_* launch needs nbytes of scratch: one buffer serves all of them (stream-ordered), allocated when the largest is known"""
+        if nbytes < 0:
+            _lib.check(-1, 'msc_mx workspace')
+        self.mx_descs.append((d, nbytes))
+
+    def place_mx_ws(self):
+        most = max([n for _, n in self.mx_descs], default=0)
+        if most:
+            ws = self.vec(most, dtype=torch.uint8)
+            for d, _ in self.mx_descs:
+                d.ws = ws.data_ptr()
 
     def slots(self, C_):
         """device address of a fresh [BN_SLOTS][C][2] f64 block of the statistics arena (forward blocks first, zeroed by the first
@@ -789,8 +844,11 @@ class _Builder:
     def grad_of(self, a):
         g = self.gbuf.get(id(a.buf))
         if g is None:
-            g = torch.zeros_like(a.buf) if _ZERO_ALLOC & 4 else torch.empty_like(a.buf)
-            self.prog.bytes += g.numel() * g.element_size()
+            if id(a.buf) in self.transient:           # the gradient of a shared activation is as short-lived as the activation, and takes its place
+                g = self.shared(self.transient[id(a.buf)], a.buf.shape[1], a.buf.shape[2], a.buf.shape[3]).buf
+            else:
+                g = torch.zeros_like(a.buf) if _ZERO_ALLOC & 4 else torch.empty_like(a.buf)
+                self.prog.bytes += g.numel() * g.element_size()
             self.gbuf[id(a.buf)] = g
             self.slices[id(g)] = self.slices.get(id(a.buf), set())
             self.prog.keep.append(g)
@@ -1022,6 +1080,8 @@ class _Builder:
                       bn.running_var.data_ptr(), BN_EPS, scale.data_ptr(), shift.data_ptr(), cout)
             self.conv(fwd, x, w, out, relu=int(relu), scale=scale, shift=shift, res=res, **geo)
             return
+        if self.ckpt and stem is None:
+            return self._conv_bn_ckpt(name, x, conv, bn, geo, relu, out, res, scale, shift)
         y = self.act(out.H, out.W, cout)
         if pend is not None:           # the producer's BatchNorm + ReLU ride on this conv's operand fetch; `x` (its activation) is written on the way
             d = self.conv_desc(Act(pend._y), w, y, want_stats=True, in_bn=pend, **geo)
@@ -1149,6 +1209,58 @@ class _Builder:
                 if not acc:
                     self.gwriter[(id(x.buf), x.c0, x.C)] = d
                 self.glast[(id(x.buf), x.c0, x.C)] = d      # ... or, as the LAST writer of a stage's output gradient (the downsample branch), a join's
+
+    def _conv_bn_ckpt(self, name, x, conv, bn, geo, relu, out, res, scale, shift):
+        """conv_bn's training form with 8-bit checkpoints: the convolution's input and its raw output are packed (E4M3) behind their last use in the forward; the
+        ReLU mask is msc_bn_apply's byte mask"""
+        net, lib, P, fwd = self.net, self.lib, self.prog, self.prog.fwd
+        cout = conv.out_channels
+        x8 = self.packed(x)
+        y = self.shared('y', out.H, out.W, cout)
+        d = self.conv_desc(x, net._pack['w'][name], y, want_stats=True, **geo)
+        d.stats = self.slots(cout)
+        self.emit(fwd, lib.msc_conv_igemm, C.byref(d))
+        mean, invstd, count, rmask = self.vec(cout), self.vec(cout), out.pixels, None
+        if relu:
+            rmask = torch.empty((self.N, out.H, out.W, cout * self.es // 16), dtype=torch.uint8, device=self.dev)
+            P.bytes += rmask.numel()
+            P.keep.append(rmask)
+        self.emit(fwd, lib.msc_bn_apply, y.ptr, y.ld, res.ptr if res is not None else None, res.ld if res is not None else 0, out.ptr, out.ld, d.stats, count,
+                  bn.weight.data_ptr(), bn.bias.data_ptr(), BN_EPS, BN_MOMENTUM, bn.running_mean.data_ptr(), bn.running_var.data_ptr(), scale.data_ptr(),
+                  shift.data_ptr(), mean.data_ptr(), invstd.data_ptr(), _p(rmask), rmask.shape[3] if relu else 0, int(relu), self.dt, count, cout)
+        y8 = self.packed(y)
+        self.ops.append(lambda: self._conv_bn_ckpt_bwd(name, x, x8, y, y8, conv, bn, geo, out, res, mean, invstd, rmask))
+
+    def _conv_bn_ckpt_bwd(self, name, x, x8, y, y8, conv, bn, geo, out, res, mean, invstd, rmask):
+        net, lib, P, bwd = self.net, self.lib, self.prog, self.prog.bwd
+        dout = self.grad_of(out)
+        d = _lib.MxBnBwdDesc()
+        d.dout, d.dout_ld, d.rows, d.C, d.dtype = dout.ptr, dout.ld, out.pixels, conv.out_channels, self.dt
+        d.y, d.y_scales, d.y_ld, d.s_ld = y8[0].data_ptr(), y8[1].data_ptr(), y8[0].shape[3], y8[1].shape[3]
+        d.gamma, d.mean, d.invstd = bn.weight.data_ptr(), mean.data_ptr(), invstd.data_ptr()
+        if rmask is not None:
+            d.relu, d.relu_mask, d.mask_ld = 3, rmask.data_ptr(), rmask.shape[3]
+        d.dy, d.dy_ld = y.ptr, y.ld               # into the shared buffer y was in
+        d.dgamma, d.dbeta, d.accumulate = self.g(bn.weight), self.g(bn.bias), 1
+        if res is not None:
+            gres = self.grad_of(res)
+            d.dres, d.dres_ld, d.dres_acc = gres.ptr, gres.ld, self.grad_acc(res)
+        self.mx_ws(d, lib.msc_mx_bn_bwd_workspace_bytes(d.rows, d.C))
+        P.keep.append(d)
+        self.emit(bwd, lib.msc_mx_bn_bwd, C.byref(d))
+        w = _lib.MxWgradDesc()
+        w.p, w.p_ld, w.dtype, w.N, w.Hp, w.Wp, w.A = y.ptr, y.ld, self.dt, self.N, y.H, y.W, y.C
+        w.q, w.q_scales, w.q_ld, w.s_ld = x8[0].data_ptr(), x8[1].data_ptr(), x8[0].shape[3], x8[1].shape[3]
+        w.Hq, w.Wq, w.B, w.KH, w.KW, w.stride, w.pad, w.accumulate = x.H, x.W, x.C, geo['KH'], geo['KW'], geo['stride'], geo['pad'], 1
+        w.dw = self.g(conv.weight)
+        self.mx_ws(w, lib.msc_mx_wgrad_workspace_bytes(C.byref(w)))
+        P.keep.append(w)
+        self.emit(bwd, lib.msc_mx_wgrad, C.byref(w))
+        gx, acc, wt, k = self.grad_of(x), self.grad_acc(x), net._pack['wt'][name], geo['KH']
+        if geo['stride'] == 1:
+            self.conv(bwd, y, wt, gx, KH=k, KW=k, stride=1, pad=geo['pad'], flip=1, res=gx if acc else None)
+        else:
+            self.conv(bwd, y, wt, gx, KH=k, KW=k, stride=2, pad=geo['pad'], mode=1, res=gx if acc else None)
 
     def stem_bn_pool(self, name, x, conv, bn, pooled, stem):
         """encoder.conv1 (7-tap x 32-wide implicit GEMM on the prepared image) + BatchNorm2d (batch statistics) + ReLU + MaxPool2d(2,2)
@@ -1381,13 +1493,13 @@ class _Builder:
                 ho, wo = hh // s, ww // s
                 planes = blk.conv1.out_channels
                 last = bi == len(blocks) - 1
-                out = skips[li] if last else self.act(ho, wo, planes * exp)
+                out = skips[li] if last else self.block_act('o%d' % (bi & 1), ho, wo, planes * exp)      # (shared: two blocks' outputs live at a time)
                 idt = cur
                 if blk.downsample is not None:
-                    idt = self.act(ho, wo, planes * exp)
+                    idt = self.block_act('o1', ho, wo, planes * exp)
                     self.conv_bn(base + '.downsample.0', cur, blk.downsample[0], blk.downsample[1], s, False, idt)
                 if net._kind == 'basic':
-                    a = self.act(ho, wo, planes)
+                    a = self.block_act('m', ho, wo, planes)
                     self.conv_bn(base + '.conv1', cur, blk.conv1, blk.bn1, s, True, a)
                     self.conv_bn(base + '.conv2', a, blk.conv2, blk.bn2, 1, True, out, res=idt)
                 elif self.bottleneck_fused(base, cur, blk, out):
@@ -1399,10 +1511,10 @@ class _Builder:
                     # layer3's 8 k-pixel maps are where it costs most (conv3 14.6 -> 21.8 us against the 3.8 us launch it saves,
                     # profiles/r5_run6_rocprofv3_kernel_stats_train_bn_on_load_all.txt); restricted to layer1 / layer2 (MSC_BN_ON_LOAD_MIN_PIXELS=30000) it is as neutral
                     on_load = self.bn_on_load and planes <= 512 and self.N * hh * ww >= self.bn_on_load_min_pixels
-                    a = self.act(hh, ww, planes)
+                    a = self.block_act('m', hh, ww, planes)
                     pend1 = self.conv_bn(base + '.conv1', cur, blk.conv1, blk.bn1, 1, True, a,
                                          defer=on_load and s == 1 and ww % 16 == 0 and hh % 8 == 0 and _os_env.environ.get('MSC_BN_ON_LOAD_3X3', '1') != '0')
-                    b = self.act(ho, wo, planes)
+                    b = self.block_act('m', ho, wo, planes)
                     # MSC_BN_ON_LOAD_1X1=0: conv2 (the 3x3 halo kernel: the pass is amortised over nine taps, on its natural tile) applies bn1 on load,
                     # conv3 reads a materialised activation (its pass costs more than the launch it saves, profiles/r5_run1_bn_on_load_ab.txt)
                     pend2 = self.conv_bn(base + '.conv2', a, blk.conv2, blk.bn2, s, True, b,
@@ -1470,6 +1582,7 @@ class _Builder:
             for op in reversed(self.ops):
                 op()
             self.flush_wgrads()
+            self.place_mx_ws()
             P.bwd[zero_at] = (lib.msc_memset_zero, (self.slot_arena.data_ptr() + 8 * bwd_slots_from, 8 * (self.slot_used - bwd_slots_from)))
         P.keep += [xp]
         P.acts = {'c1': s1, 'd0': d0, 'cat2': cat2, 'cat3': cat3, 'cat4': cat4, 'cat5': cat5}

@@ -143,8 +143,8 @@ def test_linear_refusals_and_workspace():
     refused(run(x=None), 'x (or its codes')
     refused(run(x=None, x_codes=A16, x_scales=A16, xc_ld=16, xs_ld=2), 'x (or its codes')
     assert run(M=0) == 0
-    many = dict(M=1000, K=256, N=3000, x_ld=256, w_ld=128, s_ld=8, out_ld=3000)
-    assert lib.msc_mx_linear_workspace_bytes(C.byref(linear_desc(**many))) >= 1000 * (128 + 8)
+    many = dict(M=1000, K=4096, N=3000, x_ld=4096, w_ld=2048, s_ld=128, out_ld=3000)      # x is packed by a launch of its own
+    assert lib.msc_mx_linear_workspace_bytes(C.byref(linear_desc(**many))) >= 1000 * (2048 + 128)
     refused(run(ws=None, **many), 'workspace')
     refused(run(ws=A16 + 4, **many), 'workspace')
     assert lib.msc_mx_linear_workspace_bytes(C.byref(linear_desc(x=None, **many))) == 0
@@ -219,3 +219,11 @@ def test_oracle_batchnorm_gradient_against_differences():
         e = np.eye(3)[c] * h
         assert abs((f(y, gamma + e, beta) - f(y, gamma - e, beta)) / (2 * h) - dgamma[c]) < 1e-7
         assert abs((f(y, gamma, beta + e) - f(y, gamma, beta - e)) / (2 * h) - dbeta[c]) < 1e-7
+
+
+def test_network_option_is_checked():
+    from mapping_challenge_amd.unet_models import UNetResNet
+    with pytest.raises(ValueError, match='activation_checkpoint'):
+        UNetResNet(34, 2, num_filters=32, dropout_2d=0.0, is_deconv=True, activation_checkpoint='int8')
+    net = UNetResNet(34, 2, num_filters=32, dropout_2d=0.0, is_deconv=True, activation_checkpoint='e4m3')
+    assert net.activation_checkpoint == 'e4m3'
