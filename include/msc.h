@@ -555,8 +555,8 @@ int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream);
 
 /* pointwise convolution / linear layer on E2M1 operands (v_mfma_scale_f32_16x16x128_f8f6f4), fp32 accumulation:
  *   out[m][n] = act(scale[n] * sum_k x[m][k]*w[n][k] + shift[n] + res[m][n]);   scale / shift / res may be NULL
- * x: `dtype`, quantised within the call, or already packed (x NULL; x_codes / x_scales).  out and res have `dtype`; res may be out.
- * x_ld, out_ld, res_ld in elements, the others in bytes.  ws: msc_mx_linear_workspace_bytes(d) bytes (may be 0), 16-byte aligned. */
+ * x: `dtype`, quantised within the call, or already packed (x NULL; x_codes / x_scales).  out and res have `dtype`; res may be out, x may not.
+ * x_ld, out_ld, res_ld in elements, the others in bytes.  ws: msc_mx_linear_workspace_bytes(d) bytes of the same descriptor (may be 0), 16-byte aligned. */
 typedef struct msc_mx_linear_desc {
     const void* x;
     const uint8_t* x_codes;

@@ -567,6 +567,7 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_linear: w needs 16-byte aligned rows of whole E2M1 blocks and one scale byte per block");
     if (d->x && (d->x_ld < d->K || (uintptr_t)d->x % es))
         return msc_fail(MSC_ERR_ARG, "msc_mx_linear: x misaligned or row pitch %lld below %d channels", (long long)d->x_ld, d->K);
+    if (d->x == d->out || d->x_codes == d->out) return msc_fail(MSC_ERR_ARG, "msc_mx_linear: out cannot be x: other channels' blocks still read it");
     if (!d->x && !packed_ok(d->x_codes, d->xc_ld, d->x_scales, d->xs_ld, d->K, E2M1::BYTES))
         return msc_fail(MSC_ERR_ARG, "msc_mx_linear: x (or its codes: 16-byte aligned rows of whole E2M1 blocks, and scales) missing");
     if (p.bytes && (!d->ws || (uintptr_t)d->ws & 15)) return msc_fail(MSC_ERR_ARG, "msc_mx_linear: workspace missing or not 16-byte aligned");

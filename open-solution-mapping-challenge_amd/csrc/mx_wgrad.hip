@@ -436,6 +436,9 @@ extern "C" int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream) {
     if ((int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * (p.ta / 32) * (p.tb / 32) >= 1ll << 30 ||
         (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * p.splits >= 1ll << 30)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 tiles or more");
+    const int64_t hw = (int64_t)d->Hp * d->Wp, image = (int64_t)d->Hq * d->Wq * (d->q_ld > d->s_ld ? d->q_ld : d->s_ld);
+    if (((p.chunk - 1) / hw + 2) * image >= 1ll << 31)
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: the images of %d output pixels span 2 GiB", p.chunk);
     WgArgs a;
     a.p = (const char*)d->p; a.q = d->q; a.qs = d->q_scales; a.dw = d->dw; a.part = (float*)d->ws;
     a.p_ld = d->p_ld; a.q_ld = d->q_ld; a.s_ld = d->s_ld;

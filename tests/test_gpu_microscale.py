@@ -142,6 +142,33 @@ def test_weight_gradient_of_rows(rows, a, b, dtype):
     assert got.shape == (a, 1, 1, b) and (np.abs(got - ref) <= tol).all(), np.abs(got - ref).max()
 
 
+def test_weight_gradient_of_small_numbers():
+    """fp16 below its normal range: the checkpoint holds multiples of 2^-24, and they count"""
+    saved, x = packed((500, 40), 'e4m3', 19, 'fp16', 2e-6)
+    assert (np.abs(x) < 2.0 ** -14).mean() > 0.9 and (x != 0).mean() > 0.9
+    dy = values((500, 24), 'fp16', 20).cuda()
+    got, ref, tol = check_wgrad(dy, saved, x, 1, 1, 0, 'fp16')
+    assert (np.abs(got - ref) <= tol).all(), np.abs(got - ref).max()
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('n,h,w,a,b,k,stride', [(5, 40, 44, 130, 70, 3, 1), (8, 64, 64, 256, 64, 1, 1), (3, 50, 30, 64, 130, 3, 2), (1200, 3, 2, 128, 128, 3, 1)])
+def test_weight_gradient_of_many_pixels(n, h, w, a, b, k, stride, dtype):
+    """several pixel ranges, two wave groups to a block, images smaller than a step; the sums by a float64 product on the device"""
+    from mapping_challenge_amd import microscale as mx
+    saved, x = packed((n, h * stride, w * stride, b), 'e4m3', 21, dtype)
+    dy = values((n, h, w, a), dtype, 22, 1e-2).cuda()
+    got = mx.conv_weight_grad(dy, saved, kernel=k, stride=stride, pad=k // 2).double()
+    xp = torch.nn.functional.pad(torch.from_numpy(x).cuda(), (0, 0, k // 2, k // 2 + stride, k // 2, k // 2 + stride))
+    d = dy.double().flatten(0, 2).t().contiguous()
+    for i in range(k):
+        for j in range(k):
+            q = xp[:, i:i + h * stride:stride, j:j + w * stride:stride].reshape(-1, b).contiguous()
+            ref, mag = d @ q, d.abs() @ q.abs()
+            assert ((got[:, i, j] - ref).abs() <= (n * h * w + 2) * U * mag + 1e-37).all()
+            assert float((got[:, i, j] - ref).norm() / ref.norm()) < 2e-6
+
+
 def test_weight_gradient_accumulates_slices_and_repeats():
     from mapping_challenge_amd import microscale as mx
     saved, x = packed((2, 16, 16, 64), 'e4m3', 15)
@@ -301,7 +328,7 @@ def quantised(x, dtype):
 
 @pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
 @pytest.mark.parametrize('m,k,n', [(1, 1, 1), (1, 32, 5), (2, 33, 64), (1, 2100, 130), (5, 1024, 200), (15, 31, 17), (16, 256, 64), (17, 520, 65), (40, 100, 300),
-                                   (64, 64, 64), (129, 96, 128), (300, 300, 130), (130, 4096, 40)])
+                                   (64, 64, 64), (129, 96, 128), (300, 300, 130), (130, 4096, 40), (16, 8000, 40), (2, 120000, 20), (600, 1030, 520)])
 def test_linear(m, k, n, dtype):
     from mapping_challenge_amd import microscale as mx
     x = values((m, k), dtype, m + k).cuda()
@@ -315,6 +342,29 @@ def test_linear(m, k, n, dtype):
     buf = res.clone()
     assert mx.linear(x, w, scale=scale, shift=shift, res=buf, relu=True, out=buf) is buf         # the residual in place
     assert torch.equal(buf, mx.linear(x, w, scale=scale, shift=shift, res=res, relu=True))
+
+
+@pytest.mark.parametrize('dtype,m,k,n', [('bf16', 2100, 300, 2100), ('fp16', 4113, 72, 4100), ('bf16', 4113, 1100, 4100), ('fp32', 2100, 1100, 2100)])
+def test_linear_tiles(dtype, m, k, n):
+    """the large tiles: several per block, ragged in every direction, scale rows off the dword, a lost block of x and of w"""
+    from mapping_challenge_amd import microscale as mx
+    x = values((m, k), dtype, 81).cuda()
+    w, wv = packed((n, k), 'e2m1', 82, 'fp32', 0.1)
+    g = torch.Generator().manual_seed(9)
+    scale, shift, res = torch.rand(n, generator=g).cuda() + 0.5, torch.randn(n, generator=g).cuda(), values((m, n), dtype, 83).cuda()
+    xv = quantised(x, dtype)
+    got = mx.linear(x, w, scale=scale, shift=shift, res=res, relu=True)
+    lin_check(got, xv, wv, dtype, scale, shift, res, True)
+    assert torch.equal(got, mx.linear(mx.pack(x, 'e2m1'), w, scale=scale, shift=shift, res=res, relu=True))
+    buf = res.clone()
+    assert torch.equal(got, mx.linear(x, w, scale=scale, shift=shift, res=buf, relu=True, out=buf))
+    x[m - 1, k - 1] = float('inf')
+    w.scales[n - 1, 0] = 255
+    got = torch.isnan(mx.linear(x, w))
+    assert got[m - 1].all() and got[:, n - 1].all() and got.sum() == m + n - 1
+    with pytest.raises(Exception, match='cannot be x'):
+        y = torch.zeros((m, m), dtype=DT[dtype], device='cuda')
+        mx.linear(y, mx.pack(torch.zeros((m, m), device='cuda'), 'e2m1'), out=y)
 
 
 @pytest.mark.parametrize('m', [3, 200])

@@ -69,6 +69,9 @@ def test_weight_gradient_refusals_and_workspace():
     for bad in (dict(KH=0), dict(KW=17), dict(stride=0), dict(stride=17), dict(pad=-1), dict(pad=17)):
         refused(run(**bad), 'kernel')
     refused(run(N=1 << 20, Hp=64, Wp=64), '2^30')
+    refused(run(q_ld=1 << 24), '2^28')
+    refused(run(p_ld=1 << 24), '2^24')
+    refused(run(N=200, Hp=1, Wp=1, Hq=16, Wq=16, KH=16, KW=16, pad=0, q_ld=1 << 19), '2 GiB')
     for bad in (dict(p=None), dict(dw=None), dict(p_ld=63), dict(p=A16 + 1), dict(dw=A16 + 2)):
         refused(run(**bad), 'tensor')
     for bad in (dict(q=None), dict(q=A16 + 4), dict(q_ld=32), dict(q_ld=68), dict(s_ld=1), dict(q_scales=None)):
@@ -119,7 +122,7 @@ def test_batchnorm_refusals_and_workspace():
 
 def linear_desc(**kw):
     d = _lib.MxLinearDesc()
-    v = dict(x=A16, w=A16, w_scales=A16, out=A16, ws=A16, x_ld=64, w_ld=32, s_ld=2, out_ld=48, M=5, dtype=_lib.BF16, K=64, N=48)
+    v = dict(x=A16, w=A16, w_scales=A16, out=2 * A16, ws=A16, x_ld=64, w_ld=32, s_ld=2, out_ld=48, M=5, dtype=_lib.BF16, K=64, N=48)
     for k, x in dict(v, **kw).items():
         setattr(d, k, x)
     return d
@@ -135,7 +138,8 @@ def test_linear_refusals_and_workspace():
         assert lib.msc_mx_linear_workspace_bytes(C.byref(linear_desc(**bad))) == -1
     for bad in (dict(out=None), dict(out_ld=47), dict(out=A16 + 1), dict(res=A16, res_ld=40), dict(res=A16 + 1, res_ld=48)):
         refused(run(**bad), 'out')
-    refused(run(res=A16, res_ld=64, out_ld=48), 'in place')
+    refused(run(res=2 * A16, out=2 * A16, res_ld=64, out_ld=48), 'in place')
+    refused(run(out=A16, x=A16), 'cannot be x')
     for bad in (dict(w=None), dict(w=A16 + 8), dict(w_ld=16), dict(s_ld=1), dict(w_scales=None)):
         refused(run(**bad), 'E2M1')
     refused(run(x_ld=63), 'x misaligned')
