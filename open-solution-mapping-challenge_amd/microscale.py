@@ -27,34 +27,70 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 class MxTensor:
     """A packed tensor of shape [..., channels]: codes uint8 [..., blocks * 32 (E4M3) or 16 (E2M1)], scales uint8 [..., blocks], blocks = ceil(channels / 32).
     Rows of codes start on 16 bytes; both may be slices of wider buffers."""
-    __slots__ = ('codes', 'scales', 'channels', 'fmt')
+    __slots__ = ('_codes', '_scales', '_buf', '_lead', 'channels', 'fmt')
 
-    def __init__(self, codes, scales, channels, fmt='e4m3', check=True):
-        self.codes, self.scales, self.channels, self.fmt = codes, scales, channels, fmt
-        if not check:
-            return
+    def __init__(self, codes, scales, channels, fmt='e4m3'):
         if fmt not in FORMATS:
             raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
         nb = (channels + 31) // 32
         if channels <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise ValueError('a packed tensor has at least one channel, and uint8 codes and scales')
-        if codes.shape[-1] != nb * FORMATS[fmt][1] or scales.shape[-1] != nb or codes.shape[:-1] != scales.shape[:-1]:
+        lead = codes.shape[:-1]
+        if codes.shape[-1] != nb * FORMATS[fmt][1] or scales.shape[-1] != nb or lead != scales.shape[:-1]:
             raise ValueError('%d channels in %s take %d code bytes and %d scales per row, got codes %s and scales %s'
                              % (channels, fmt, nb * FORMATS[fmt][1], nb, tuple(codes.shape), tuple(scales.shape)))
         if codes.device != scales.device:
             raise ValueError('codes and scales are on different devices')
+        self._codes, self._scales, self._buf, self._lead, self.channels, self.fmt = codes, scales, None, lead, channels, fmt
+
+    @classmethod
+    def _made(cls, buf, lead, channels, fmt):
+        """over one allocation, the codes and then the scales; the two tensors are made when somebody asks for them (each costs the host what a launch does)"""
+        t = cls.__new__(cls)
+        t._codes, t._scales, t._buf, t._lead, t.channels, t.fmt = None, None, buf, lead, channels, fmt
+        return t
+
+    def _split(self):
+        nb, per = (self.channels + 31) // 32, FORMATS[self.fmt][1]
+        n = self._buf.numel() // (per + 1) * per
+        self._codes, self._scales = self._buf[:n].view(self._lead + (nb * per,)), self._buf[n:].view(self._lead + (nb,))
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._split()
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._split()
+        return self._scales
 
     @property
     def shape(self):
-        return self.codes.shape[:-1] + (self.channels,)
+        return self._lead + (self.channels,)
 
     @property
     def device(self):
-        return self.codes.device
+        return (self._codes if self._buf is None else self._buf).device
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self._codes.numel() + self._scales.numel() if self._buf is None else self._buf.numel()
+
+    def _args(self, what):
+        """rows, address and row pitch of the codes, of the scales"""
+        buf = self._buf
+        if buf is None:
+            codes, scales = self._codes, self._scales
+            rows, c_ld = _rows(codes, what)
+            return rows, codes.data_ptr(), c_ld, scales.data_ptr(), _rows(scales, what)[1]
+        if not buf.is_cuda:
+            raise _lib.MscError('%s: needs a CUDA/ROCm tensor; there is no CPU path in the product' % what)
+        nb, per = (self.channels + 31) // 32, FORMATS[self.fmt][1]
+        rows, at = buf.numel() // (nb * (per + 1)), buf.data_ptr()
+        return rows, at, nb * per, at + rows * nb * per, nb
 
 
 def _rows(t, what):
@@ -129,10 +165,12 @@ def _workspace(nbytes, like, name):
 
 def empty(shape, fmt='e4m3', device='cuda'):
     """an uninitialised MxTensor of `shape` [..., channels]"""
-    nb = (shape[-1] + 31) // 32
-    lead = tuple(shape[:-1])
-    return MxTensor(torch.empty(lead + (nb * FORMATS[fmt][1],), dtype=torch.uint8, device=device),
-                    torch.empty(lead + (nb,), dtype=torch.uint8, device=device), shape[-1], fmt)
+    lead, c = torch.Size(shape[:-1]), shape[-1]
+    if fmt not in FORMATS:
+        raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
+    if c <= 0:
+        raise ValueError('a packed tensor has at least one channel')
+    return MxTensor._made(torch.empty(lead.numel() * ((c + 31) // 32) * (FORMATS[fmt][1] + 1), dtype=torch.uint8, device=device), lead, c, fmt)
 
 
 def pack(x, fmt='e4m3', out=None):
@@ -141,38 +179,35 @@ def pack(x, fmt='e4m3', out=None):
     if fmt not in FORMATS:
         raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
     rows, ld = _rows(x, 'pack')
-    dt, shape, dev = _dtype(x, 'pack'), x.shape, x.device
-    c = shape[-1]
-    fid, nbytes = FORMATS[fmt]
+    shape, dev = x.shape, x.device
+    c, (fid, per) = shape[-1], FORMATS[fmt]
     if out is None:
         if c <= 0:
-            raise ValueError('pack: no channels')
+            raise ValueError('a packed tensor has at least one channel')
         nb = (c + 31) // 32
-        c_ld, s_ld = nb * nbytes, nb
-        codes = torch.empty(shape[:-1] + (c_ld,), dtype=torch.uint8, device=dev)
-        scales = codes.new_empty(shape[:-1] + (nb,))
-        out = MxTensor(codes, scales, c, fmt, False)
+        buf = torch.empty(rows * nb * (per + 1), dtype=torch.uint8, device=dev)
+        out = MxTensor._made(buf, shape[:-1], c, fmt)
+        cp, c_ld, s_ld = buf.data_ptr(), nb * per, nb
+        sp = cp + rows * c_ld
     else:
-        if out.shape != tuple(shape) or out.fmt != fmt:
-            raise ValueError('pack: out holds %s in %s, not %s in %s' % (out.shape, out.fmt, tuple(shape), fmt))
-        codes, scales = out.codes, out.scales
-        _same_device('pack', dev, codes)
-        c_ld, s_ld = _rows(codes, 'pack')[1], _rows(scales, 'pack')[1]
-    _run('msc_mx_pack', dev, x.data_ptr(), ld, dt, codes.data_ptr(), c_ld, scales.data_ptr(), s_ld, fid, rows, c)
+        if out.shape != shape or out.fmt != fmt:
+            raise ValueError('pack: out holds %s in %s, not %s in %s' % (tuple(out.shape), out.fmt, tuple(shape), fmt))
+        _same_device('pack', dev, out)
+        _, cp, c_ld, sp, s_ld = out._args('pack')
+    _run('msc_mx_pack', dev, x.data_ptr(), ld, _dtype(x, 'pack'), cp, c_ld, sp, s_ld, fid, rows, c)
     return out
 
 
 def unpack(t, dtype=torch.bfloat16, out=None):
     """the values an MxTensor stands for, in `dtype` (any of the three; the one that was packed holds every value exactly)"""
-    codes, scales, dev = t.codes, t.scales, t.codes.device
-    rows, c_ld = _rows(codes, 'unpack')
+    rows, cp, c_ld, sp, s_ld = t._args('unpack')
+    dev, c = t.device, t.channels
     if out is None:
-        out, ld = torch.empty(t.shape, dtype=dtype, device=dev), t.channels
+        out, ld = torch.empty(t._lead + (c,), dtype=dtype, device=dev), c
     else:
         _out(out, t.shape, out.dtype, dev, 'unpack')
         ld = _rows(out, 'unpack')[1]
-    _run('msc_mx_unpack', dev, codes.data_ptr(), c_ld, scales.data_ptr(), _rows(scales, 'unpack')[1], FORMATS[t.fmt][0], out.data_ptr(), ld,
-         _dtype(out, 'unpack'), rows, t.channels)
+    _run('msc_mx_unpack', dev, cp, c_ld, sp, s_ld, FORMATS[t.fmt][0], out.data_ptr(), ld, _dtype(out, 'unpack'), rows, c)
     return out
 
 
@@ -186,11 +221,10 @@ def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=
         raise ValueError('conv_weight_grad: accumulate needs out')
     kh, kw = (kernel, kernel) if isinstance(kernel, int) else kernel
     rows, p_ld = _rows(dy, 'conv_weight_grad')
-    _, q_ld = _rows(saved.codes, 'conv_weight_grad')
-    _, s_ld = _rows(saved.scales, 'conv_weight_grad')
+    _, qp, q_ld, sp, s_ld = saved._args('conv_weight_grad')
     a, b = dy.shape[-1], saved.channels
     if kh == 1 and kw == 1 and stride == 1 and pad == 0:
-        if dy.shape[:-1] != saved.codes.shape[:-1]:
+        if dy.shape[:-1] != saved._lead:
             raise ValueError('conv_weight_grad: dy %s and input %s differ in their rows' % (tuple(dy.shape), tuple(saved.shape)))
         n, hp, wp, hq, wq = rows, 1, 1, 1, 1
     else:
@@ -205,8 +239,8 @@ def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=
         out = torch.empty((a, kh, kw, b), dtype=torch.float32, device=dev)
     elif not _out(out, (a, kh, kw, b), torch.float32, dev, 'conv_weight_grad').is_contiguous():
         raise ValueError('conv_weight_grad: out has to be contiguous')
-    _same_device('conv_weight_grad', dev, saved.codes)
-    d = _lib.MxWgradDesc(dy.data_ptr(), saved.codes.data_ptr(), saved.scales.data_ptr(), out.data_ptr(), None, p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad'),
+    _same_device('conv_weight_grad', dev, saved)
+    d = _lib.MxWgradDesc(dy.data_ptr(), qp, sp, out.data_ptr(), None, p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad'),
                          n, hp, wp, a, hq, wq, b, kh, kw, stride, pad, accumulate)
     ref = C.byref(d)
     ws = _workspace(_lib.load().msc_mx_wgrad_workspace_bytes(ref), dy, 'msc_mx_wgrad_workspace_bytes')
@@ -227,10 +261,10 @@ def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=N
         raise ValueError('batchnorm_backward: dout %s and input %s differ' % (tuple(dout.shape), tuple(saved.shape)))
     if (scale is None) != (shift is None) or (scale is not None and relu_mask is not None):
         raise ValueError('batchnorm_backward: the ReLU takes relu_mask, or scale and shift, or neither')
-    dev, c, codes, scales = dout.device, saved.channels, saved.codes, saved.scales
+    dev, c = dout.device, saved.channels
     rows, dout_ld = _rows(dout, 'batchnorm_backward')
-    y_ld, s_ld = _rows(codes, 'batchnorm_backward')[1], _rows(scales, 'batchnorm_backward')[1]
-    _same_device('batchnorm_backward', dev, codes, relu_mask)
+    _, yp, y_ld, sp, s_ld = saved._args('batchnorm_backward')
+    _same_device('batchnorm_backward', dev, saved, relu_mask)
     dt, dtype = _dtype(dout, 'batchnorm_backward'), dout.dtype
     relu, mask_ld = 0, 0
     if relu_mask is not None:
@@ -248,7 +282,7 @@ def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=N
     dbeta = dgamma.new_empty(c)
     dres = torch.empty(dout.shape, dtype=dtype, device=dev) if residual else None
     ws = _workspace(_lib.load().msc_mx_bn_bwd_workspace_bytes(rows, c), dout, 'msc_mx_bn_bwd_workspace_bytes')
-    d = _lib.MxBnBwdDesc(dout.data_ptr(), codes.data_ptr(), scales.data_ptr(), relu_mask.data_ptr() if relu_mask is not None else None,
+    d = _lib.MxBnBwdDesc(dout.data_ptr(), yp, sp, relu_mask.data_ptr() if relu_mask is not None else None,
                          _vector(gamma, c, dev, 'batchnorm_backward: gamma'), _vector(mean, c, dev, 'batchnorm_backward: mean'),
                          _vector(invstd, c, dev, 'batchnorm_backward: invstd'), _vector(scale, c, dev, 'batchnorm_backward: scale'),
                          _vector(shift, c, dev, 'batchnorm_backward: shift'), dgamma.data_ptr(), dbeta.data_ptr(), dy.data_ptr(),
@@ -265,17 +299,17 @@ def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=N
     packed = isinstance(x, MxTensor)
     if w.fmt != 'e2m1' or (packed and x.fmt != 'e2m1'):
         raise ValueError('linear: the operands have to be in e2m1')
-    wc, k = w.codes, w.channels
-    if wc.dim() != 2 or k != x.shape[-1]:
+    k = w.channels
+    if len(w._lead) != 1 or k != x.shape[-1]:
         raise ValueError('linear: x %s and w %s do not go together' % (tuple(x.shape), tuple(w.shape)))
-    dev, n = x.device, wc.shape[0]
+    dev, (n,) = x.device, w._lead
     if dtype is None:
         dtype = x.dtype if not packed else out.dtype if out is not None else res.dtype if res is not None else torch.bfloat16
     if not packed and x.dtype != dtype:
         raise ValueError('linear: the result has the type of x')
     if packed:
-        m, xc_ld = _rows(x.codes, 'linear')
-        xp, x_ld, xcp, xsp, xs_ld = None, 0, x.codes.data_ptr(), x.scales.data_ptr(), _rows(x.scales, 'linear')[1]
+        m, xcp, xc_ld, xsp, xs_ld = x._args('linear')
+        xp, x_ld = None, 0
     else:
         m, x_ld = _rows(x, 'linear')
         xp, xcp, xsp, xc_ld, xs_ld = x.data_ptr(), None, None, 0, 0
@@ -284,15 +318,16 @@ def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=N
         out, out_ld = torch.empty(shape, dtype=dtype, device=dev), n
     else:
         out_ld = _rows(_out(out, shape, dtype, dev, 'linear'), 'linear')[1]
-    _same_device('linear', dev, wc)
+    _same_device('linear', dev, w)
     resp, res_ld = (None, 0) if res is None else (res.data_ptr(), _rows(_out(res, shape, dtype, dev, 'linear: res'), 'linear')[1])
     if m == 0:
         return out
-    d = _lib.MxLinearDesc(xp, xcp, xsp, wc.data_ptr(), w.scales.data_ptr(), _vector(scale, n, dev, 'linear: scale'), _vector(shift, n, dev, 'linear: shift'), resp,
-                          out.data_ptr(), None, x_ld, xc_ld, xs_ld, _rows(wc, 'linear')[1], _rows(w.scales, 'linear')[1], res_ld, out_ld, m,
+    _, wp, w_ld, wsp, ws_ld = w._args('linear')
+    d = _lib.MxLinearDesc(xp, xcp, xsp, wp, wsp, _vector(scale, n, dev, 'linear: scale'), _vector(shift, n, dev, 'linear: shift'), resp,
+                          out.data_ptr(), None, x_ld, xc_ld, xs_ld, w_ld, ws_ld, res_ld, out_ld, m,
                           _dtype(out, 'linear'), k, n, relu)
     ref = C.byref(d)
-    ws = _workspace(_lib.load().msc_mx_linear_workspace_bytes(ref), wc, 'msc_mx_linear_workspace_bytes')
+    ws = _workspace(_lib.load().msc_mx_linear_workspace_bytes(ref), w, 'msc_mx_linear_workspace_bytes')
     if ws is not None:
         d.ws = ws.data_ptr()
     _run('msc_mx_linear', dev, ref)
