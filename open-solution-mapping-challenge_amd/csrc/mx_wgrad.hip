@@ -7,6 +7,11 @@
 // a power of two is a bf16 / fp16 / f32 number, so the matrix instructions see exactly what was stored): half the bytes of the
 // 16-bit input come from HBM, and the conversion is one instruction for two elements, once per block.  The k-contiguous fragments come out of LDS by
 // transposing reads.  The pixel ranges' partial tiles go to the workspace, tile by tile and coalesced, and a second launch adds them in order.
+//
+// What bounds it.  131072 pixels, 256 x 64: HBM (75 MB, 16.5 + 4 us with the join, 19.2 us a call = 4.0 TB/s).  32x16x16, 256 -> 256, 3x3 (9.7 GFLOP, 6 us of
+// matrix instructions): latency -- nine steps a group; of 24 us some 9 are launch, first loads and partial sums, and loads, LDS writes, reads and products
+// of a step take about as long as each other and overlap in part.  Divisions in the loop, the depth of the prefetch and the share of VALU
+// work were tried out of it one by one: within 3 %.
 #include <type_traits>
 
 #include "common.h"
@@ -251,10 +256,10 @@ template <typename T, int TA, int TB, int KG, bool VECP> __global__ __launch_bou
     put(smem, even);
     if (steps > 2) fetch(2, even);
     __syncthreads();
-    auto step = [&](int s, Regs& r) {                                  // r: step s + 1, which goes to the half last read two barriers ago
-        compute(smem + (s & 1) * L::STAGE);
-        if (s + 1 < steps) put(smem + ((s + 1) & 1) * L::STAGE, r);
+    auto step = [&](int s, Regs& r) {                                  // r: step s + 1, which goes to the half that was multiplied before the last barrier
+        if (s + 1 < steps) put(smem + ((s + 1) & 1) * L::STAGE, r);    // before the products, so that they cover it (3x3: 25.4 -> 23.9 us)
         if (s + 3 < steps) fetch(s + 3, r);
+        compute(smem + (s & 1) * L::STAGE);
         __syncthreads();
     };
     for (int s = 0; s < steps; s += 2) {
