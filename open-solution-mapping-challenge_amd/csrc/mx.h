@@ -88,22 +88,53 @@ static inline FastDiv fast_div(unsigned d) {
 __device__ __forceinline__ unsigned div_of(unsigned n, const FastDiv& f) { return (unsigned)(((unsigned long long)n * f.m) >> 31 >> f.s); }
 
 // 8 consecutive elements of a row as floats: 16-byte loads, or one element at a time below `left` of them (the others zero)
-template <typename T> __device__ __forceinline__ void load8(const T* p, float* v) {
+// Elements of a row as they are stored, 16 bytes a unit, eight elements a chunk.  Whole units move at any alignment of their elements (the hardware's global
+// accesses take it), so that odd widths and channel slices need no kernels of their own; the last unit of a row comes element by element, every
+// load issued before the first is waited for.  Kept raw until they are used: converted at once, each load would be waited for before the next one goes out.
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
+template <typename T> __device__ __forceinline__ uint4 load_unit(const T* p, int left) {
+    constexpr int N = Vec16<T>::N;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (left >= N) {
+        v = __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4_any*>(p));
+    } else if (left > 0) {
+        unsigned e[N];
 #pragma unroll
-    for (int i = 0; i < 8; i += Vec16<T>::N) Vec16<T>::load(p + i, v + i);
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(T) == 2) e[i] = *reinterpret_cast<const uint16_t*>(p + min(i, left - 1));
+            else e[i] = *reinterpret_cast<const unsigned*>(p + min(i, left - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = i < left ? e[i] : 0u;
+        if constexpr (sizeof(T) == 2) v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        else v = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+    return v;
 }
-template <typename T> __device__ __forceinline__ void load8_some(const T* p, int left, float* v) {
+template <typename T> struct Chunk {
+    static constexpr int UNITS = sizeof(T) / 2;
+    uint4 v[UNITS];
+    __device__ __forceinline__ void floats(float* f) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? ElemIO<T>::load(p + i) : 0.f;
+        for (int k = 0; k < UNITS; ++k) Vec16<T>::unpack(v[k], f + k * Vec16<T>::N);
+    }
+};
+template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T* p, int left) {
+    Chunk<T> c;
+#pragma unroll
+    for (int k = 0; k < c.UNITS; ++k) c.v[k] = load_unit<T>(p + k * Vec16<T>::N, left - k * Vec16<T>::N);
+    return c;
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, const float* v) {
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, int left, const float* v) {
+    constexpr int N = Vec16<T>::N;
+    if (left >= 8) {
 #pragma unroll
-    for (int i = 0; i < 8; i += Vec16<T>::N) Vec16<T>::store(p + i, v + i);
-}
-template <typename T> __device__ __forceinline__ void store8_some(T* p, int left, const float* v) {
+        for (int k = 0; k < 8 / N; ++k) *reinterpret_cast<u32x4_any*>(p + k * N) = __builtin_bit_cast(u32x4_any, Vec16<T>::pack(v + k * N));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < left) ElemIO<T>::store(p + i, v[i]);
+        for (int i = 0; i < 8; ++i)
+            if (i < left) ElemIO<T>::store(p + i, v[i]);
+    }
 }
 
 // one quad's block of 32: `v` the 8 elements of this lane, raw.  Returns the scale byte; q = the elements in units of the scale, zeros in a NaN block

@@ -15,28 +15,25 @@ constexpr int64_t MAX_CHUNKS = 1ll << 30;      // 8-channel chunks of one launch
 
 // ------------------------------------------------------------------------------------------------ pack
 // A lane takes 8 consecutive channels of a row, a quad of lanes a block: the maximum over the block is two DPP steps, loads (16 bytes a lane for the
-// 16-bit types) and code stores (8 or 4 bytes) are contiguous over the wave.  Four chunks per lane are in flight.  VEC: rows start on 16 bytes
-// and chunks that are whole are loaded as vectors; otherwise element by element (odd widths, channel slices at odd offsets).
-template <typename F, typename T, bool VEC>
+// 16-bit types) and code stores (8 or 4 bytes) are contiguous over the wave.  Four chunks per lane are in flight.
+template <typename F, typename T>
 __global__ void pack_kernel(const T* __restrict__ x, long x_ld, uint8_t* __restrict__ codes, long codes_ld, uint8_t* __restrict__ scales, long scales_ld,
                             unsigned chunks, FastDiv per_row, int C) {
     const unsigned first = blockIdx.x * (unsigned)SPAN + threadIdx.x;
-    float v[UNROLL][8];
+    Chunk<T> in[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const unsigned id = first + u * THREADS;
         const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
-        const int left = id < chunks ? C - (int)(k * 8) : 0;
-        const T* p = x + (long)row * x_ld + k * 8;
-        if (VEC && left >= 8) load8<T>(p, v[u]);
-        else load8_some<T>(p, left, v[u]);
+        in[u] = load_chunk<T>(x + (long)row * x_ld + k * 8, id < chunks ? C - (int)(k * 8) : 0);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const unsigned id = first + u * THREADS;
         const unsigned row = div_of(id, per_row), k = id - row * per_row.d;
-        float q[8];
-        const unsigned e = block_scale<F, T>(v[u], q);
+        float v[8], q[8];
+        in[u].floats(v);
+        const unsigned e = block_scale<F, T>(v, q);
         if (id >= chunks) continue;              // whole quads: `chunks` is a multiple of four
         uint8_t* c = codes + (long)row * codes_ld + k * (F::BYTES / 4);
         if (F::ID == 0) *reinterpret_cast<uint2*>(c) = encode8_e4m3(q);
@@ -45,7 +42,7 @@ __global__ void pack_kernel(const T* __restrict__ x, long x_ld, uint8_t* __restr
     }
 }
 
-template <typename F, typename T, bool VEC>
+template <typename F, typename T>
 __global__ void unpack_kernel(const uint8_t* __restrict__ codes, long codes_ld, const uint8_t* __restrict__ scales, long scales_ld, T* __restrict__ out,
                               long out_ld, unsigned chunks, FastDiv per_row, int C) {
     const unsigned first = blockIdx.x * (unsigned)SPAN + threadIdx.x;
@@ -69,26 +66,21 @@ __global__ void unpack_kernel(const uint8_t* __restrict__ codes, long codes_ld, 
         float v[8];
         if (F::ID == 0) { decode4_e4m3(w[u].x, s, v); decode4_e4m3(w[u].y, s, v + 4); }
         else decode8_e2m1(w[u].x, s, v);
-        const int left = C - (int)(k * 8);
-        T* p = out + (long)row * out_ld + k * 8;
-        if (VEC && left >= 8) store8<T>(p, v);
-        else store8_some<T>(p, left, v);
+        store_chunk<T>(out + (long)row * out_ld + k * 8, C - (int)(k * 8), v);
     }
 }
 
 template <typename F, typename T>
-void launch_pack(const void* x, long x_ld, uint8_t* codes, long codes_ld, uint8_t* scales, long scales_ld, unsigned chunks, unsigned per_row, int C, bool vec,
+void launch_pack(const void* x, long x_ld, uint8_t* codes, long codes_ld, uint8_t* scales, long scales_ld, unsigned chunks, unsigned per_row, int C,
                  hipStream_t st) {
     const dim3 grid((chunks + SPAN - 1) / SPAN);
-    auto k = vec ? pack_kernel<F, T, true> : pack_kernel<F, T, false>;
-    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, st, (const T*)x, x_ld, codes, codes_ld, scales, scales_ld, chunks, fast_div(per_row), C);
+    hipLaunchKernelGGL((pack_kernel<F, T>), grid, dim3(THREADS), 0, st, (const T*)x, x_ld, codes, codes_ld, scales, scales_ld, chunks, fast_div(per_row), C);
 }
 template <typename F, typename T>
 void launch_unpack(const uint8_t* codes, long codes_ld, const uint8_t* scales, long scales_ld, void* out, long out_ld, unsigned chunks, unsigned per_row, int C,
-                   bool vec, hipStream_t st) {
+                   hipStream_t st) {
     const dim3 grid((chunks + SPAN - 1) / SPAN);
-    auto k = vec ? unpack_kernel<F, T, true> : unpack_kernel<F, T, false>;
-    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, st, codes, codes_ld, scales, scales_ld, (T*)out, out_ld, chunks, fast_div(per_row), C);
+    hipLaunchKernelGGL((unpack_kernel<F, T>), grid, dim3(THREADS), 0, st, codes, codes_ld, scales, scales_ld, (T*)out, out_ld, chunks, fast_div(per_row), C);
 }
 
 int mx_check(const char* name, const void* x, int64_t x_ld, int dtype, const void* codes, int64_t codes_ld, const void* scales, int64_t scales_ld, int fmt,
@@ -119,12 +111,11 @@ extern "C" int msc_mx_pack(const void* x, int64_t x_ld, int dtype, uint8_t* code
     int rc = mx_check("msc_mx_pack", x, x_ld, dtype, codes, codes_ld, scales, scales_ld, fmt, rows, C);
     if (rc || rows == 0) return rc;
     const unsigned per_row = (unsigned)((C + BLOCK - 1) / BLOCK) * 4;
-    const bool vec = vec_ok(x, x_ld, dtype);
     const int64_t rows_max = MAX_CHUNKS / per_row;
     for (int64_t r = 0; r < rows; r += rows_max) {
         const int64_t n = rows - r < rows_max ? rows - r : rows_max;
         const char* xr = (const char*)x + r * x_ld * msc_dtype_size(dtype);
-#define MX_ARGS (xr, x_ld, codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, (unsigned)(n * per_row), per_row, C, vec, (hipStream_t)stream)
+#define MX_ARGS (xr, x_ld, codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, (unsigned)(n * per_row), per_row, C, (hipStream_t)stream)
         if (fmt == MSC_MX_E4M3) MX_BY_TYPE(E4M3, launch_pack);
         else MX_BY_TYPE(E2M1, launch_pack);
 #undef MX_ARGS
@@ -137,12 +128,11 @@ extern "C" int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8
     int rc = mx_check("msc_mx_unpack", out, out_ld, dtype, codes, codes_ld, scales, scales_ld, fmt, rows, C);
     if (rc || rows == 0) return rc;
     const unsigned per_row = (unsigned)((C + BLOCK - 1) / BLOCK) * 4;
-    const bool vec = vec_ok(out, out_ld, dtype);
     const int64_t rows_max = MAX_CHUNKS / per_row;
     for (int64_t r = 0; r < rows; r += rows_max) {
         const int64_t n = rows - r < rows_max ? rows - r : rows_max;
         char* o = (char*)out + r * out_ld * msc_dtype_size(dtype);
-#define MX_ARGS (codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, o, out_ld, (unsigned)(n * per_row), per_row, C, vec, (hipStream_t)stream)
+#define MX_ARGS (codes + r * codes_ld, codes_ld, scales + r * scales_ld, scales_ld, o, out_ld, (unsigned)(n * per_row), per_row, C, (hipStream_t)stream)
         if (fmt == MSC_MX_E4M3) MX_BY_TYPE(E4M3, launch_unpack);
         else MX_BY_TYPE(E2M1, launch_unpack);
 #undef MX_ARGS
@@ -172,11 +162,9 @@ struct BnArgs {
 };
 
 // what one chunk (8 channels of a row) reads, and its masked gradients and centred inputs: apart, so that several rows' loads are in flight
-struct BnRaw { float d[8]; uint2 y; unsigned e, bits; };
-template <typename T, int RELU, bool VEC> __device__ __forceinline__ void bn_read(const BnArgs& a, long row, int c0, int left, BnRaw& r) {
-    const T* d = (const T*)a.dout + row * a.dout_ld + c0;
-    if (VEC && left >= 8) load8<T>(d, r.d);
-    else load8_some<T>(d, left, r.d);
+template <typename T> struct BnRaw { Chunk<T> d; uint2 y; unsigned e, bits; };
+template <typename T, int RELU> __device__ __forceinline__ void bn_read(const BnArgs& a, long row, int c0, int left, BnRaw<T>& r) {
+    r.d = load_chunk<T>((const T*)a.dout + row * a.dout_ld + c0, left);
     r.y = *reinterpret_cast<const uint2*>(a.y + row * a.y_ld + c0);
     r.e = a.y_scales[row * a.s_ld + (c0 >> 5)];
     r.bits = 0xff;
@@ -186,21 +174,21 @@ template <typename T, int RELU, bool VEC> __device__ __forceinline__ void bn_rea
         else r.bits = (m[c0 >> 2] & 15u) | (left > 4 ? (unsigned)m[(c0 >> 2) + 1] << 4 : 0u);
     }
 }
-template <int RELU> __device__ __forceinline__ void bn_terms(const BnRaw& r, const float* mean, const float* sc, const float* sh, float* dh, float* t) {
+template <typename T, int RELU> __device__ __forceinline__ void bn_terms(const BnRaw<T>& r, const float* mean, const float* sc, const float* sh, float* dh, float* t) {
     const float s = scale_value(r.e);
     float y[8];
     decode4_e4m3(r.y.x, s, y);
     decode4_e4m3(r.y.y, s, y + 4);
+    r.d.floats(dh);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        dh[i] = r.d[i];
         if (RELU == 2) dh[i] = fmaf(sc[i], y[i], sh[i]) > 0.f ? dh[i] : 0.f;
         if (RELU == 3) dh[i] = (r.bits >> i) & 1 ? dh[i] : 0.f;
         t[i] = y[i] - mean[i];
     }
 }
 
-template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
+template <typename T, int RELU> __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
     __shared__ float2 red[THREADS][9];         // 8 channels per thread, one column of padding
     const int cols = 1 << a.cols_log2;
     const int col = threadIdx.x & (cols - 1), rg = threadIdx.x >> a.cols_log2, groups = THREADS >> a.cols_log2;
@@ -213,24 +201,24 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
         sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
         sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
     }
-    auto add = [&](const BnRaw& raw) {
+    auto add = [&](const BnRaw<T>& raw) {
         float dh[8], t[8];
-        bn_terms<RELU>(raw, mean, sc, sh, dh, t);
+        bn_terms<T, RELU>(raw, mean, sc, sh, dh, t);
 #pragma unroll
         for (int i = 0; i < 8; ++i) { s1[i] += dh[i]; s2[i] = fmaf(dh[i], t[i], s2[i]); }
     };
     if (left > 0) {
         for (long r = (long)blockIdx.x * BN_ROWS * groups + rg; r < a.rows; r += (long)a.strips * BN_ROWS * groups) {
             if (r + (BN_ROWS - 1) * groups < a.rows) {
-                BnRaw raw[BN_ROWS];
+                BnRaw<T> raw[BN_ROWS];
 #pragma unroll
-                for (int k = 0; k < BN_ROWS; ++k) bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw[k]);
+                for (int k = 0; k < BN_ROWS; ++k) bn_read<T, RELU>(a, r + k * groups, c0, left, raw[k]);
 #pragma unroll
                 for (int k = 0; k < BN_ROWS; ++k) add(raw[k]);
             } else {
                 for (int k = 0; k < BN_ROWS && r + k * groups < a.rows; ++k) {
-                    BnRaw raw;
-                    bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw);
+                    BnRaw<T> raw;
+                    bn_read<T, RELU>(a, r + k * groups, c0, left, raw);
                     add(raw);
                 }
             }
@@ -295,10 +283,10 @@ __global__ __launch_bounds__(256) void bn_finish_kernel(BnArgs a) {
 }
 
 // the results of one chunk
-template <typename T, int RELU, bool VEC>
-__device__ __forceinline__ void bn_store(const BnArgs& a, long r, int c0, int left, const BnRaw& raw, const float4* f, const float* mean, const float* sc, const float* sh) {
+template <typename T, int RELU>
+__device__ __forceinline__ void bn_store(const BnArgs& a, long r, int c0, int left, const BnRaw<T>& raw, const float4* f, const float* mean, const float* sc, const float* sh) {
     float dh[8], t[8];
-    bn_terms<RELU>(raw, mean, sc, sh, dh, t);
+    bn_terms<T, RELU>(raw, mean, sc, sh, dh, t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = fmaf(f[i].x, dh[i], fmaf(f[i].z, t[i], f[i].y));
     T* o = (T*)a.dy + r * a.dy_ld + c0;
@@ -306,19 +294,16 @@ __device__ __forceinline__ void bn_store(const BnArgs& a, long r, int c0, int le
         T* g = (T*)a.dres + r * a.dres_ld + c0;
         if (a.dres_acc) {
             float old[8];
-            if (VEC && left >= 8) load8<T>(g, old);
-            else load8_some<T>(g, left, old);
+            load_chunk<T>(g, left).floats(old);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dh[i] += old[i];
         }
-        if (VEC && left >= 8) store8<T>(g, dh);
-        else store8_some<T>(g, left, dh);
+        store_chunk<T>(g, left, dh);
     }
-    if (VEC && left >= 8) store8<T>(o, t);
-    else store8_some<T>(o, left, t);
+    store_chunk<T>(o, left, t);
 }
 
-template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
+template <typename T, int RELU> __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
     const int cols = 1 << a.cols_log2;
     const int col = threadIdx.x & (cols - 1), rg = threadIdx.x >> a.cols_log2, groups = THREADS >> a.cols_log2;
     const int c0 = (blockIdx.y * cols + col) * 8, left = a.C - c0;
@@ -334,16 +319,16 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
     }
     for (long r = (long)blockIdx.x * BN_APPLY_ROWS * groups + rg; r < a.rows; r += (long)gridDim.x * BN_APPLY_ROWS * groups) {
         if (r + (BN_APPLY_ROWS - 1) * groups < a.rows) {               // (all the rows' loads before the first store: the outputs may be dout itself)
-            BnRaw raw[BN_APPLY_ROWS];
+            BnRaw<T> raw[BN_APPLY_ROWS];
 #pragma unroll
-            for (int k = 0; k < BN_APPLY_ROWS; ++k) bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw[k]);
+            for (int k = 0; k < BN_APPLY_ROWS; ++k) bn_read<T, RELU>(a, r + k * groups, c0, left, raw[k]);
 #pragma unroll
-            for (int k = 0; k < BN_APPLY_ROWS; ++k) bn_store<T, RELU, VEC>(a, r + k * groups, c0, left, raw[k], f, mean, sc, sh);
+            for (int k = 0; k < BN_APPLY_ROWS; ++k) bn_store<T, RELU>(a, r + k * groups, c0, left, raw[k], f, mean, sc, sh);
         } else {
             for (int k = 0; k < BN_APPLY_ROWS && r + k * groups < a.rows; ++k) {
-                BnRaw raw;
-                bn_read<T, RELU, VEC>(a, r + k * groups, c0, left, raw);
-                bn_store<T, RELU, VEC>(a, r + k * groups, c0, left, raw, f, mean, sc, sh);
+                BnRaw<T> raw;
+                bn_read<T, RELU>(a, r + k * groups, c0, left, raw);
+                bn_store<T, RELU>(a, r + k * groups, c0, left, raw, f, mean, sc, sh);
             }
         }
     }
@@ -353,7 +338,7 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(256) void
 // blocks.  (2048 x 512 fp16: three launches of 4.5 + 3.4 + 4.1 us, whose host time alone was 20 us, against one.)
 constexpr int BN_FEW_THREADS = 512, BN_FEW_COLS = 2, BN_FEW_GROUPS = BN_FEW_THREADS / BN_FEW_COLS, BN_FEW_PER = 8, BN_FEW = BN_FEW_GROUPS * BN_FEW_PER;
 
-template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(BN_FEW_THREADS) void bn_few_rows_kernel(BnArgs a) {
+template <typename T, int RELU> __global__ __launch_bounds__(BN_FEW_THREADS) void bn_few_rows_kernel(BnArgs a) {
     __shared__ float2 red[BN_FEW_THREADS][9];
     __shared__ double2 part[BN_FEW_THREADS];
     __shared__ float4 coef[16];
@@ -367,17 +352,16 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(BN_FEW_TH
         sc[i] = RELU == 2 && i < left ? a.scale[c0 + i] : 0.f;
         sh[i] = RELU == 2 && i < left ? a.shift[c0 + i] : 0.f;
     }
-    BnRaw raw[BN_FEW_PER];
+    BnRaw<T> raw[BN_FEW_PER];
+    if (left > 0) {
 #pragma unroll
-    for (int k = 0; k < BN_FEW_PER; ++k) {
-        const long r = rg + k * BN_FEW_GROUPS;
-        if (r < a.rows && left > 0) bn_read<T, RELU, VEC>(a, r, c0, left, raw[k]);
+        for (int k = 0; k < BN_FEW_PER; ++k) bn_read<T, RELU>(a, min((long)rg + k * BN_FEW_GROUPS, a.rows - 1), c0, left, raw[k]);       // (no branch between the loads)
     }
 #pragma unroll
     for (int k = 0; k < BN_FEW_PER; ++k) {
         if (rg + k * BN_FEW_GROUPS >= a.rows || left <= 0) continue;
         float dh[8], t[8];
-        bn_terms<RELU>(raw[k], mean, sc, sh, dh, t);
+        bn_terms<T, RELU>(raw[k], mean, sc, sh, dh, t);
 #pragma unroll
         for (int i = 0; i < 8; ++i) { s1[i] += dh[i]; s2[i] = fmaf(dh[i], t[i], s2[i]); }
     }
@@ -413,7 +397,7 @@ template <typename T, int RELU, bool VEC> __global__ __launch_bounds__(BN_FEW_TH
     for (int i = 0; i < 8; ++i) f[i] = coef[col * 8 + i];
 #pragma unroll
     for (int k = 0; k < BN_FEW_PER; ++k)
-        if (rg + k * BN_FEW_GROUPS < a.rows) bn_store<T, RELU, VEC>(a, rg + k * BN_FEW_GROUPS, c0, left, raw[k], f, mean, sc, sh);
+        if (rg + k * BN_FEW_GROUPS < a.rows) bn_store<T, RELU>(a, rg + k * BN_FEW_GROUPS, c0, left, raw[k], f, mean, sc, sh);
 }
 
 struct BnPlan { int cols_log2, ctiles, strips, apply_strips; };
@@ -433,20 +417,20 @@ BnPlan bn_plan(int64_t rows, int C) {
     return p;
 }
 
-template <typename T, int RELU> void bn_launch(const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
+template <typename T, int RELU> void bn_launch(const BnArgs& a, const BnPlan& p, hipStream_t st) {
     if (a.rows <= BN_FEW) {
-        hipLaunchKernelGGL((vec ? bn_few_rows_kernel<T, RELU, true> : bn_few_rows_kernel<T, RELU, false>), dim3((a.C + 15) / 16), dim3(BN_FEW_THREADS), 0, st, a);
+        hipLaunchKernelGGL((bn_few_rows_kernel<T, RELU>), dim3((a.C + 15) / 16), dim3(BN_FEW_THREADS), 0, st, a);
         return;
     }
     const dim3 grid(p.strips, p.ctiles), apply_grid(p.apply_strips, p.ctiles);
-    hipLaunchKernelGGL((vec ? bn_reduce_kernel<T, RELU, true> : bn_reduce_kernel<T, RELU, false>), grid, dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((bn_reduce_kernel<T, RELU>), grid, dim3(THREADS), 0, st, a);
     hipLaunchKernelGGL(bn_finish_kernel, dim3((a.C + FIN - 1) / FIN), dim3(THREADS), 0, st, a);
-    hipLaunchKernelGGL((vec ? bn_apply_kernel<T, RELU, true> : bn_apply_kernel<T, RELU, false>), apply_grid, dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((bn_apply_kernel<T, RELU>), apply_grid, dim3(THREADS), 0, st, a);
 }
-template <typename T> void bn_by_relu(int relu, const BnArgs& a, const BnPlan& p, bool vec, hipStream_t st) {
-    if (relu == 0) bn_launch<T, 0>(a, p, vec, st);
-    else if (relu == 2) bn_launch<T, 2>(a, p, vec, st);
-    else bn_launch<T, 3>(a, p, vec, st);
+template <typename T> void bn_by_relu(int relu, const BnArgs& a, const BnPlan& p, hipStream_t st) {
+    if (relu == 0) bn_launch<T, 0>(a, p, st);
+    else if (relu == 2) bn_launch<T, 2>(a, p, st);
+    else bn_launch<T, 3>(a, p, st);
 }
 
 }  // namespace
@@ -484,10 +468,9 @@ extern "C" int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream) {
     a.coef = (float4*)d->ws; a.part = (double2*)((char*)d->ws + (int64_t)d->C * 16);
     a.dout_ld = d->dout_ld; a.y_ld = d->y_ld; a.s_ld = d->s_ld; a.mask_ld = d->mask_ld; a.dy_ld = d->dy_ld; a.dres_ld = d->dres_ld;
     a.rows = d->rows; a.C = d->C; a.strips = p.strips; a.cols_log2 = p.cols_log2; a.accumulate = d->accumulate; a.dres_acc = d->dres_acc;
-    const bool vec = vec_ok(d->dout, d->dout_ld, d->dtype) && vec_ok(d->dy, d->dy_ld, d->dtype) && (!d->dres || vec_ok(d->dres, d->dres_ld, d->dtype));
     hipStream_t st = (hipStream_t)stream;
-    if (d->dtype == MSC_F32) bn_by_relu<float>(d->relu, a, p, vec, st);
-    else if (d->dtype == MSC_BF16) bn_by_relu<bf16_t>(d->relu, a, p, vec, st);
-    else bn_by_relu<f16_t>(d->relu, a, p, vec, st);
+    if (d->dtype == MSC_F32) bn_by_relu<float>(d->relu, a, p, st);
+    else if (d->dtype == MSC_BF16) bn_by_relu<bf16_t>(d->relu, a, p, st);
+    else bn_by_relu<f16_t>(d->relu, a, p, st);
     return msc_check_launch("msc_mx_bn_bwd");
 }

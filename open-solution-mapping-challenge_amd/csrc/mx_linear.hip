@@ -32,9 +32,7 @@ __device__ __forceinline__ i32x8 fp4_operand(uint4 v) { return i32x8{(int)v.x, (
 
 // eight consecutive channels from n: their scale / shift; one row's residual, and its results.  Apart, because res may be out: a loop that loads and stores row by
 // row could not have the next row's load in flight
-template <typename T, bool VEC> struct Epilogue {
-    static constexpr int PIECES = sizeof(T) / 2;
-    struct Res { uint4 v[PIECES]; };
+template <typename T> struct Epilogue {
     float sc[8], sh[8];
     int n, left;
     __device__ __forceinline__ Epilogue(const LinArgs& a, int n_) : n(n_), left(a.N - n_) {
@@ -44,36 +42,17 @@ template <typename T, bool VEC> struct Epilogue {
             sh[i] = a.shift && i < left ? a.shift[n + i] : 0.f;
         }
     }
-    __device__ __forceinline__ Res load(const LinArgs& a, long m, bool in) const {
-        Res r;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) r.v[k] = make_uint4(0, 0, 0, 0);
-        if (!a.res || left <= 0 || !in) return r;
-        const T* p = (const T*)a.res + m * a.res_ld + n;
-        if (VEC && left >= 8) {
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) r.v[k] = reinterpret_cast<const uint4*>(p)[k];
-        } else {
-            float v[8];
-            load8_some<T>(p, left, v);
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) r.v[k] = Vec16<T>::pack(v + k * Vec16<T>::N);
-        }
-        return r;
-    }
-    __device__ __forceinline__ void store(const LinArgs& a, long m, bool in, const Res& res, const float* v) const {
+    __device__ __forceinline__ Chunk<T> load(const LinArgs& a, long m, bool in) const { return load_chunk<T>((const T*)a.res + m * a.res_ld + n, a.res && in ? left : 0); }
+    __device__ __forceinline__ void store(const LinArgs& a, long m, bool in, const Chunk<T>& res, const float* v) const {
         if (left <= 0 || !in) return;
         float r[8];
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) Vec16<T>::unpack(res.v[k], r + k * Vec16<T>::N);
+        res.floats(r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float y = fmaf(v[i], sc[i], sh[i]) + r[i];
             r[i] = a.relu && y < 0.f ? 0.f : y;                        // NaN stays NaN
         }
-        T* o = (T*)a.out + m * a.out_ld + n;
-        if (VEC && left >= 8) store8<T>(o, r);
-        else store8_some<T>(o, left, r);
+        store_chunk<T>((T*)a.out + m * a.out_ld + n, left, r);
     }
 };
 
@@ -151,15 +130,14 @@ template <int FM, int TM> __device__ __forceinline__ void lin_step(const LinArgs
 // bytes of each of 16 rows.  Neighbours pl, pl ^ 1 swap halves first: the even lane takes channels 8 g of both rows, the odd lane channels 32 + 8 g, and an
 // instruction writes whole 128-byte lines of eight rows (131072 x 64 -> 256: 28.0 ->
 // 25.8 us)
-template <typename T, int FM, bool VEC>
+template <typename T, int FM>
 __device__ __forceinline__ void lin_write(const LinArgs& a, long m0, int last_m, int n0, int wm, int wn, int g, int pl, const f32x4 (&acc)[FM][4]) {
-    using E = Epilogue<T, VEC>;
     const bool odd = pl & 1;
-    const E ep(a, n0 + wn * 64 + (odd ? 32 : 0) + 8 * g);
+    const Epilogue<T> ep(a, n0 + wn * 64 + (odd ? 32 : 0) + 8 * g);
     constexpr int ROWS = FM < 4 ? FM : 4;
 #pragma unroll
     for (int i0 = 0; i0 < FM; i0 += ROWS) {
-        typename E::Res r0[ROWS], r1[ROWS];
+        Chunk<T> r0[ROWS], r1[ROWS];
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
             const int m = wm * (FM * 16) + (i0 + k) * 16 + (pl & ~1);
@@ -183,7 +161,7 @@ __device__ __forceinline__ void lin_write(const LinArgs& a, long m0, int last_m,
     }
 }
 
-template <typename T, int WM, int WN, int FM, bool VEC>
+template <typename T, int WM, int WN, int FM>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(LinArgs a) {
     constexpr int WAVES = WM * WN, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN;
     constexpr int DX = TM / 8 / WAVES, DW = TN / 8 / WAVES;            // DMA instructions (8 rows of codes each) per wave and step
@@ -261,7 +239,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(LinArgs a) {
             lin_step<FM, TM>(a, s, smem + half * STAGE, SCALES, wm, wn, g, pl, acc);
             half ^= 1;
         }
-        lin_write<T, FM, VEC>(a, here.m0, here.last_m, here.n0, wm, wn, g, pl, acc);
+        lin_write<T, FM>(a, here.m0, here.last_m, here.n0, wm, wn, g, pl, acc);
         here = next;
     }
 }
@@ -269,8 +247,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(LinArgs a) {
 // ------------------------------------------------------------------------------------------------ few channels
 // The same tile, with x quantised on the way into LDS instead of by a launch of its own: for weights of a few tiles' channels, where every row of x is then
 // quantised once or a few times.  x comes through registers (a quad of lanes a block, as in packing), w by LDS-DMA.  WM x WN = 4 waves, FM fragments of rows each.
-template <typename T, int WM, int WN, int FM, bool VEC>
-__global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xin, long xin_ld, int xvec) {
+template <typename T, int WM, int WN, int FM>
+__global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xin, long xin_ld) {
     constexpr int WAVES = 4, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN, DW = TN / 8 / WAVES, DSW = (TN / 32 + WAVES - 1) / WAVES;
     constexpr int SCALES = ROWS * ROWB, STAGE = SCALES + ROWS * 8, CHUNKS = TM * UNITS * 4 / 256;
     static_assert(WM * WN == WAVES && 2 * STAGE <= 80 * 1024, "two blocks per CU");
@@ -298,31 +276,18 @@ __global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xi
     };
     // chunk i of thread t: eight channels, number t % 32 of a step, of row t / 32 + 8 i
     const int xr = tid >> 5, xc = tid & 31;
-    constexpr int PIECES = sizeof(T) / 2;                              // 16-byte pieces of a chunk, kept as they were loaded
-    uint4 xv[CHUNKS][PIECES];
+    Chunk<T> xv[CHUNKS];
     auto fetch = [&](int s) {
-        const int k = s * (UNITS * BLOCK) + xc * 8, left = a.K - k;
+        const int k = s * (UNITS * BLOCK) + xc * 8;
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const T* p = xin + (m0 + min(xr + 8 * i, last_m)) * xin_ld + k;
-            if (xvec && left >= 8) {
-#pragma unroll
-                for (int k = 0; k < PIECES; ++k) xv[i][k] = reinterpret_cast<const uint4*>(p)[k];
-            } else {
-                float v[8];
-                load8_some<T>(p, left, v);
-#pragma unroll
-                for (int k = 0; k < PIECES; ++k) xv[i][k] = Vec16<T>::pack(v + k * Vec16<T>::N);
-            }
-        }
+        for (int i = 0; i < CHUNKS; ++i) xv[i] = load_chunk<T>(xin + (m0 + min(xr + 8 * i, last_m)) * xin_ld + k, a.K - k);
     };
     auto put = [&](char* st) {
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
             const int r = xr + 8 * i, b = xc >> 2;
             float v[8], q[8];
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) Vec16<T>::unpack(xv[i][k], v + k * Vec16<T>::N);
+            xv[i].floats(v);
             const unsigned e = block_scale<E2M1, T>(v, q);
             *reinterpret_cast<unsigned*>(st + r * ROWB + (b ^ ((r >> 1) & 7)) * 16 + (xc & 3) * 4) = encode8_e2m1(q);
             if ((xc & 3) == 0) st[SCALES + r * 8 + b] = (char)e;
@@ -348,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xi
         lin_step<FM, TM>(a, s, now, SCALES, wm, wn, g, pl, acc);
         if (s + 1 < steps) put(next);
     }
-    lin_write<T, FM, VEC>(a, m0, last_m, n0, wm, wn, g, pl, acc);
+    lin_write<T, FM>(a, m0, last_m, n0, wm, wn, g, pl, acc);
 }
 
 // scales in rows a multiple of four bytes apart, for the kernel above
@@ -367,7 +332,7 @@ static int64_t few_lds(int64_t M, int64_t nb) {          // of the fused form: c
     return M * (pad * 17 + 16) + FEW_WAVES * 64 * 16;
 }
 
-template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREADS) void mx_few_rows_kernel(LinArgs a, const T* xin, long xin_ld, int xvec) {
+template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREADS) void mx_few_rows_kernel(LinArgs a, const T* xin, long xin_ld) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, pl = lane & 15;
     const int n0 = blockIdx.x * 16;
@@ -395,11 +360,9 @@ template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREA
     if constexpr (FUSED) {
         const int per_row = nbp * 4;
         for (int id = tid; id < M * per_row; id += FEW_THREADS) {      // whole quads
-            const int m = id / per_row, k = id - m * per_row, left = a.K - k * 8;
+            const int m = id / per_row, k = id - m * per_row;
             float v[8], q[8];
-            const T* p = xin + (long)m * xin_ld + k * 8;
-            if (xvec && left >= 8) load8<T>(p, v);
-            else load8_some<T>(p, left, v);
+            load_chunk<T>(xin + (long)m * xin_ld + k * 8, a.K - k * 8).floats(v);
             const unsigned e = block_scale<E2M1, T>(v, q);
             *reinterpret_cast<unsigned*>(xc + m * pitch + k * 4) = encode8_e2m1(q);
             if ((k & 3) == 0) xsc[m * nbp + (k >> 2)] = (char)e;
@@ -489,7 +452,7 @@ int lin_check(const msc_mx_linear_desc* d) {
     return MSC_OK;
 }
 
-template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, bool vec, hipStream_t st) {
+template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, hipStream_t st) {
     constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS), RESIDENT = 256 * (LDS > 80 * 1024 ? 1 : LDS > 40 * 1024 ? 2 : 4);
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
@@ -498,7 +461,7 @@ template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, b
     if (tiles >= 1ll << 30) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^30 tiles or more");
     if (TM * a.x_ld >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TM * a.xs_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
-    auto k = vec ? mx_gemm_kernel<T, WM, WN, FM, true> : mx_gemm_kernel<T, WM, WN, FM, false>;
+    auto k = mx_gemm_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return msc_fail(MSC_ERR_HIP, "msc_mx_linear: %s", hipGetErrorString(e));
@@ -506,45 +469,44 @@ template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, b
     hipLaunchKernelGGL(k, dim3((unsigned)(tiles < RESIDENT ? tiles : RESIDENT)), dim3(WM * WN * 64), LDS, st, b);
     return MSC_OK;
 }
-template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs& a, const msc_mx_linear_desc* d, bool vec, hipStream_t st) {
+template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs& a, const msc_mx_linear_desc* d, hipStream_t st) {
     constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS);
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
     const int64_t tiles = (a.M + TM - 1) / TM * b.tiles_n;
     if (tiles >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^31 tiles or more, or a tile's rows span 2 GiB");
-    auto k = vec ? mx_fused_kernel<T, WM, WN, FM, true> : mx_fused_kernel<T, WM, WN, FM, false>;
+    auto k = mx_fused_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return msc_fail(MSC_ERR_HIP, "msc_mx_linear: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), LDS, st, b, (const T*)d->x, (long)d->x_ld, (int)vec_ok(d->x, d->x_ld, d->dtype));
+    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), LDS, st, b, (const T*)d->x, (long)d->x_ld);
     return MSC_OK;
 }
-template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const msc_mx_linear_desc* d, bool vec, hipStream_t st) {
+template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const msc_mx_linear_desc* d, hipStream_t st) {
     const dim3 few((unsigned)((a.N + 15) / 16));
     const long none = 0;
     if (p.fused) {
-        hipLaunchKernelGGL((mx_few_rows_kernel<T, 1, true>), few, dim3(FEW_THREADS), (size_t)few_lds(a.M, a.nb), st, a, (const T*)d->x, (long)d->x_ld,
-                           (int)vec_ok(d->x, d->x_ld, d->dtype));
+        hipLaunchKernelGGL((mx_few_rows_kernel<T, 1, true>), few, dim3(FEW_THREADS), (size_t)few_lds(a.M, a.nb), st, a, (const T*)d->x, (long)d->x_ld);
         return MSC_OK;
     }
     if (p.few) {
         const int fm = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
         auto k = fm == 1 ? mx_few_rows_kernel<T, 1, false> : fm == 2 ? mx_few_rows_kernel<T, 2, false> : mx_few_rows_kernel<T, 4, false>;
-        hipLaunchKernelGGL(k, few, dim3(FEW_THREADS), (size_t)fm * FEW_WAVES * 64 * 16, st, a, (const T*)nullptr, none, 0);
+        hipLaunchKernelGGL(k, few, dim3(FEW_THREADS), (size_t)fm * FEW_WAVES * 64 * 16, st, a, (const T*)nullptr, none);
         return MSC_OK;
     }
     auto tiles = [&](int tm, int tn) { return (a.M + tm - 1) / tm * ((a.N + tn - 1) / tn); };
     if (p.tile) {
-        if (a.N <= 64) return lin_launch_fused<T, 4, 1, 1>(a, d, vec, st);
-        if (a.N <= 128) return lin_launch_fused<T, 2, 2, 2>(a, d, vec, st);
-        if (p.tile_rows == 1) return lin_launch_fused<T, 1, 4, 1>(a, d, vec, st);
-        return lin_launch_fused<T, 1, 4, 2>(a, d, vec, st);
+        if (a.N <= 64) return lin_launch_fused<T, 4, 1, 1>(a, d, st);
+        if (a.N <= 128) return lin_launch_fused<T, 2, 2, 2>(a, d, st);
+        if (p.tile_rows == 1) return lin_launch_fused<T, 1, 4, 1>(a, d, st);
+        return lin_launch_fused<T, 1, 4, 2>(a, d, st);
     }
-    if (tiles(256, 256) >= 256) return lin_launch<T, 2, 4, 8>(a, vec, st);
-    if (tiles(128, 128) >= 256) return lin_launch<T, 2, 2, 4>(a, vec, st);
-    return lin_launch<T, 2, 1, 2>(a, vec, st);
+    if (tiles(256, 256) >= 256) return lin_launch<T, 2, 4, 8>(a, st);
+    if (tiles(128, 128) >= 256) return lin_launch<T, 2, 2, 4>(a, st);
+    return lin_launch<T, 2, 1, 2>(a, st);
 }
 
 }  // namespace
@@ -591,8 +553,7 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
     a.w = d->w; a.w_ld = d->w_ld;
     a.scale = d->scale; a.shift = d->shift; a.res = d->res; a.out = d->out;
     a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_m = a.tiles_n = 0;
-    const bool vec = vec_ok(d->out, d->out_ld, d->dtype) && (!d->res || vec_ok(d->res, d->res_ld, d->dtype));
     hipStream_t st = (hipStream_t)stream;
-    rc = d->dtype == MSC_F32 ? lin_by_tile<float>(a, p, d, vec, st) : d->dtype == MSC_BF16 ? lin_by_tile<bf16_t>(a, p, d, vec, st) : lin_by_tile<f16_t>(a, p, d, vec, st);
+    rc = d->dtype == MSC_F32 ? lin_by_tile<float>(a, p, d, st) : d->dtype == MSC_BF16 ? lin_by_tile<bf16_t>(a, p, d, st) : lin_by_tile<f16_t>(a, p, d, st);
     return rc ? rc : msc_check_launch("msc_mx_linear");
 }

@@ -161,15 +161,7 @@ template <typename T, int TA, int TB, int KG, bool VECP> __global__ __launch_bou
             for (int i = 0; i < L::IA; ++i) {
                 const int idx = i * THREADS + tid, row = idx / L::UA, c = a0 + idx % L::UA * L::PE;
                 const char* src = at + (long)row * a.p_ld * L::ES + idx % L::UA * 16;
-                unsigned t[4] = {0, 0, 0, 0};
-                if (row < left)
-#pragma unroll
-                    for (int k = 0; k < L::PE; ++k)
-                        if (c + k < a.A) {
-                            if (L::ES == 2) t[k >> 1] |= (unsigned)reinterpret_cast<const uint16_t*>(src)[k] << (k & 1) * 16;
-                            else t[k & 3] = reinterpret_cast<const unsigned*>(src)[k];
-                        }
-                r.p[i] = make_uint4(t[0], t[1], t[2], t[3]);
+                r.p[i] = load_unit<T>(reinterpret_cast<const T*>(src), row < left ? a.A - c : 0);
             }
         }
 #pragma unroll
