@@ -343,7 +343,10 @@ template <typename T, int RELU> __global__ __launch_bounds__(BN_FEW_THREADS) voi
     __shared__ double2 part[BN_FEW_THREADS];
     __shared__ float4 coef[16];
     const int col = threadIdx.x % BN_FEW_COLS, rg = threadIdx.x / BN_FEW_COLS;
-    const int c0 = (blockIdx.x * BN_FEW_COLS + col) * 8, left = a.C - c0;
+    // block b runs on XCD b % 8: neighbours in the channels share 128-byte lines and so an XCD's L2 (2048 x 512 fp16: 14.1 -> 9.6 us)
+    const unsigned xcd = blockIdx.x & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
+    const int place = (int)(xcd * per + min(xcd, more) + (blockIdx.x >> 3));
+    const int c0 = (place * BN_FEW_COLS + col) * 8, left = a.C - c0;
     float mean[8], sc[8], sh[8], s1[8], s2[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -387,7 +390,7 @@ template <typename T, int RELU> __global__ __launch_bounds__(BN_FEW_THREADS) voi
             }
             __syncthreads();
         }
-        const int ch = blockIdx.x * 16 + c;
+        const int ch = place * 16 + c;
         if (slice == 0) coef[c] = ch < a.C ? bn_coefficients(a, ch, s) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();
