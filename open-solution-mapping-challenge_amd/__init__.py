@@ -9,6 +9,7 @@ hand-written HIP kernels for gfx950 through the C ABI in include/msc.h (libmsc_h
   models          PyTorchUNet / PyTorchUNetWeighted (+Stream) transformers (src/models.py:50-209)
   postprocessing  the functions of src/postprocessing.py:48-258 on HIP (+ batched variants)
   tta / utils / preparation   test-time augmentation, COCO RLE + bbox encoding, target preparation on the device
+  microscale      E4M3 / E2M1 storage with block scales: pack, weight gradient and BatchNorm backward from it, linear layer
   callbacks       the reference's callback protocol for standalone use (src/steps/pytorch/callbacks.py)
   steps           Step / BaseTransformer operator API mirror (src/steps/base.py)
   pipelines       unet / unet_weighted / mask_postprocessing graphs (src/pipelines.py:12-52,248-304)

@@ -8,6 +8,12 @@
 //
 // Three forms: up to 16 (64) rows, the weights streamed once by blocks of 16 channels; a few tiles' channels, x quantised by the tile kernel itself; else packing,
 // then tiles of 256 x 256 (fewer: 128 x 128, 64 x 64).
+//
+// What bounds them.  1 x 4096 -> 4096: 6.1 us on the device for 9 MB, one wave's chain of loads; the call takes 12 us of host time.  8192 x 1024 -> 256: 12 us for
+// 21 MB, the chain of a step (read, quantise, LDS, products) on two blocks per CU.  8192 x 4096 -> 4096 with a residual: 17.5 us of packing, then 113-125 us of
+// product (275 GFLOP: 2.2-2.4 PFLOP/s).  Taken apart, its requests alone take 49 us (1 GB from the L2s at the 10-11 TB/s they deliver), reads and products
+// 45, the epilogue some 40: 134 MB of residual and result, moved by all CUs in step, with no registers left to hold a tile back (256 in use).  Requesting the
+// residual ahead of the last step spilled (160-180 us); waiting before the stores instead of behind them, 136.
 #include <type_traits>
 
 #include "common.h"
@@ -420,8 +426,8 @@ template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREA
 constexpr int FUSED_ROWS = 16, FEW_ROWS = 64;
 constexpr int64_t FUSED_LDS = 64 * 1024;
 // x quantised by the tile kernel itself (mx_fused_kernel): for weights of at most two waves' channels, and where 512 blocks of 16 (32) x 256 cover the result and the
-// reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 11.7 : 17.5; 131072 x 256 -> 64 24 : 44; 32768 x 512 -> 128 15 : 21;
-// 2048 x 512 -> 2048 12.1 : 14.1; but 8192 x 1024 -> 1024 31 : 24, 1024 x 4096 -> 1024 28 : 22, 8192 x 4096 -> 512 48 : 44
+// reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 12.4 : 17.5; 131072 x 256 -> 64 27.5 : 42.0; 32768 x 512 -> 128 15.7 : 21.9;
+// 2048 x 512 -> 2048 12.7 : 15.3; but 8192 x 1024 -> 1024 31.7 : 26.9, 1024 x 4096 -> 1024 29.5 : 22.4, 8192 x 4096 -> 512 48.4 : 43.2, 131072 x 64 -> 256 58.8 : 38.3
 constexpr int FUSED_CHANNELS = 128, FUSED_BLOCKS = 512, FUSED_K = 1024;
 
 struct LinPlan { int64_t nb, xc_ld, s_ld, codes, scales, w_scales, bytes; bool pack, fused, few, tile; int tile_rows; };      // fused: few rows, tile: few channels -- x is quantised by the product's own launch

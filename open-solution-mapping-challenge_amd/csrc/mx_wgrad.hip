@@ -100,7 +100,7 @@ template <typename T, int TA, int TB, int KG, bool VECP> __global__ __launch_bou
     const int wa = wid >> 1, wb = wid & 1, g = lane >> 4, pl = lane & 15;
     // order: the tiles of one tap and one pixel range, then the taps, then the ranges.  Block b runs on XCD b % 8.  Where a few blocks read the same pixels each XCD
     // gets a run of the order, so that they share an L2 (131072 pixels, 256 x 64, two tiles: 16.5 us against 17.8); where many do, they are spread over the
-    // XCDs: the same lines wanted by 36 blocks of one XCD at a time make a queue (32x16x16, 256 -> 256, 3x3: 29.4 us against 25.4)
+    // XCDs: the same lines wanted by 36 blocks of one XCD at a time make a queue (32x16x16, 256 -> 256, 3x3: 4 us more)
     const unsigned xcd = blockIdx.x & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
     const unsigned id = a.tiles * a.taps <= 8 ? xcd * per + min(xcd, more) + (blockIdx.x >> 3) : blockIdx.x;
     const unsigned bt = div_of(id, a.tile_div);
@@ -352,7 +352,7 @@ WgPlan wg_plan(const msc_mx_wgrad_desc* d) {
     const int64_t M = (int64_t)d->N * d->Hp * d->Wp, all = (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW;
     const int kp = d->dtype == MSC_F32 ? 32 : 64;
         // two groups of waves to a block and one block to a CU where every group has four steps to do: half the partial sums of two blocks with one group each
-    // (3x3 above: 25.4 + 5.5 us to join, against 24.7 + 7.3; 1x1: 16.5 + 4.0 against 17.3 + 4.5).  Fewer pixels: more, smaller blocks
+    // (3x3 above: 24.1 + 5.4 us to join, against 24.8 + 7.2; 1x1: 16.7 + 4.0 against 17.3 + 4.5).  Fewer pixels: more, smaller blocks
     p.kg = M * all >= 256ll * 2 * 4 * kp ? 2 : 1;
     int64_t splits = 512 / p.kg / all, most = (M + 4 * p.kg * kp - 1) / (4 * p.kg * kp);
     if (splits > most) splits = most;
