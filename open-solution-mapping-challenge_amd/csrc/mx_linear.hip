@@ -429,6 +429,7 @@ constexpr int64_t FUSED_LDS = 64 * 1024;
 // reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 12.4 : 17.5; 131072 x 256 -> 64 27.5 : 42.0; 32768 x 512 -> 128 15.7 : 21.9;
 // 2048 x 512 -> 2048 12.7 : 15.3; but 8192 x 1024 -> 1024 31.7 : 26.9, 1024 x 4096 -> 1024 29.5 : 22.4, 8192 x 4096 -> 512 48.4 : 43.2, 131072 x 64 -> 256 58.8 : 38.3
 constexpr int FUSED_CHANNELS = 128, FUSED_BLOCKS = 512, FUSED_K = 1024;
+constexpr int64_t FUSED_MOST = 1ll << 29;      // rows: 2^23 blocks, whose 2^31 threads are within a launch; the form behind the packing has a grid of the card's size
 
 struct LinPlan { int64_t nb, xc_ld, s_ld, codes, scales, w_scales, bytes; bool pack, fused, few, tile; int tile_rows; };      // fused: few rows, tile: few channels -- x is quantised by the product's own launch
 bool dword_rows(const void* s, int64_t ld) { return ((uintptr_t)s & 3) == 0 && ld % 4 == 0; }
@@ -439,7 +440,7 @@ LinPlan lin_plan(const msc_mx_linear_desc* d) {
     p.few = d->M <= FEW_ROWS;
     const int64_t tiles = (d->M + 15) / 16 * ((d->N + 255) / 256);
     p.tile_rows = tiles <= FUSED_BLOCKS ? 1 : 2;                // fragments of 16
-    p.tile = d->x && !p.few && (d->N <= FUSED_CHANNELS || (tiles <= 2 * FUSED_BLOCKS && d->K <= FUSED_K));
+    p.tile = d->x && !p.few && d->M <= FUSED_MOST && (d->N <= FUSED_CHANNELS || (tiles <= 2 * FUSED_BLOCKS && d->K <= FUSED_K));
     p.pack = d->x && !p.fused && !p.tile;
     p.xc_ld = p.nb * E2M1::BYTES;
     p.s_ld = (p.nb + 3) / 4 * 4;                               // rows of scales start on dwords
@@ -480,8 +481,7 @@ template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
     const int64_t tiles = (a.M + TM - 1) / TM * b.tiles_n;
-    if (tiles >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
-        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^31 tiles or more, or a tile's rows span 2 GiB");
+    if (TN * a.w_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
     auto k = mx_fused_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);

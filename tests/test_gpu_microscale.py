@@ -471,3 +471,43 @@ def test_tensors_of_several_devices_are_refused():
         mx.batchnorm_backward(x, t, None, torch.zeros(32), torch.ones(32, device='cuda'))
     with pytest.raises((ValueError, _lib.MscError)):
         mx.linear(x.cpu(), mx.pack(x, 'e2m1'))
+
+
+# ------------------------------------------------------------------------------------------------ past 2^31
+# Small integers: every value is its own code, products and sums stay whole numbers below 2^24 and so are exact, in any order.
+def test_rows_past_two_to_the_thirty():
+    """more rows than one launch packs or one block per 64 rows could cover"""
+    from mapping_challenge_amd import microscale as mx
+    rows = 2 ** 30 + 5
+    x = torch.tensor([1, -2, 3, 4, -6, 0, 12], dtype=torch.bfloat16, device='cuda').repeat(rows // 7 + 1)[:rows, None]
+    t = mx.pack(x, 'e2m1')
+    assert torch.equal(mx.unpack(t), x)
+    del t
+    w = mx.pack(torch.ones((1, 1), device='cuda'), 'e2m1')
+    assert torch.equal(mx.linear(x, w), x)
+
+
+def test_checkpoints_past_two_to_the_thirty_one_bytes():
+    """weight gradient and BatchNorm backward whose operands are longer than 32-bit offsets reach"""
+    from mapping_challenge_amd import microscale as mx
+    rows, c, a, part = 2 ** 26 + 7, 40, 8, 2 ** 22
+    g = torch.Generator(device='cuda').manual_seed(70)
+    x = torch.randint(-1, 2, (rows, c), dtype=torch.int8, generator=g, device='cuda').to(torch.bfloat16)
+    saved = mx.pack(x)
+    dout = torch.randint(-1, 2, (rows, c), dtype=torch.int8, generator=g, device='cuda').to(torch.bfloat16)
+    p = dout[:, :a].contiguous()
+    dw = torch.zeros((a, c), dtype=torch.float64, device='cuda')
+    for r in range(0, rows, part):
+        dw += p[r:r + part].double().t().contiguous() @ x[r:r + part].double()
+    assert torch.equal(mx.conv_weight_grad(p, saved).view(a, c).double(), dw)
+    one, zero = torch.ones(c, device='cuda'), torch.zeros(c, device='cuda')
+    dy, dgamma, dbeta = mx.batchnorm_backward(dout, saved, one, zero, one)
+    db, dg = torch.zeros(c, dtype=torch.float64, device='cuda'), torch.zeros(c, dtype=torch.float64, device='cuda')
+    for r in range(0, rows, part):
+        db += dout[r:r + part].double().sum(0)
+        dg += (dout[r:r + part].double() * x[r:r + part].double()).sum(0)
+    assert torch.equal(dbeta.double(), db) and torch.equal(dgamma.double(), dg)
+    for r in (0, rows // 2, rows - 1000):              # dy: two fused operations in fp32 and the rounding to bf16, of terms below 2
+        d, y = dout[r:r + 1000].double(), x[r:r + 1000].double()
+        ref = d - db / rows - y * (dg / rows)
+        assert ((dy[r:r + 1000].double() - ref).abs() <= ref.abs() * HALF['bf16'] + 8 * 2.0 ** -24).all()
