@@ -149,8 +149,9 @@ extern "C" int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8
 namespace {
 
 // Rows in flight per thread, and blocks.  131072 x 256 bf16 join: reduce 34.6 us with one row, 31 with two or four (3.4 TB/s: a plain read-only sum of 1 GB reaches 4.0
-// on the card), 36 with half the blocks; apply 51 with one, 42 with two (the second reading of dout and y is from the last-level cache), 48 with 8192 blocks.
-constexpr int BN_ROWS = 4, BN_APPLY_ROWS = 2, BN_BLOCKS = 1024, BN_APPLY_BLOCKS = 2048;
+// on the card), 36 with half the blocks; apply 51 with one, 42 with two (the second reading of dout and y is from the last-level cache), 40 with 4096 blocks instead of 2048, 48 with
+// 8192; the rows from the end, or on the XCD that summed them: no difference.
+constexpr int BN_ROWS = 4, BN_APPLY_ROWS = 2, BN_BLOCKS = 1024, BN_APPLY_BLOCKS = 4096;
 constexpr int BN_COLS = 32;                    // 8-channel chunks of a block's column range at most
 
 struct BnArgs {
