@@ -143,24 +143,40 @@ def _out(out, shape, dtype, dev, what):
     return out
 
 
+# Small calls are bound by the host (a launch costs it 3 us, an allocation 1.1-1.7): hence the bound entries, the stream's handle alone (the Stream object that
+# torch.cuda.current_stream() makes costs 2 us), and empty_like where a result has an operand's shape.
+_entries = {}
+
+
+def _entry(name):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    return fn
+
+
 def _run(name, dev, *args):
-    """one C call on `dev`'s current stream, with `dev` current.  (The stream's handle alone: the Stream object that torch.cuda.current_stream() makes
-    costs as much host time as a launch.)"""
-    fn = getattr(_lib.load(), name)
-    if dev.index != torch.cuda.current_device():
+    """one C call on `dev`'s current stream, with `dev` current"""
+    fn, index = _entry(name), dev.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
 
 
-def _workspace(nbytes, like, name):
-    """scratch of one call on like's device; None where it needs none"""
+def _workspace(nbytes, dev, name):
+    """scratch of one call; None where it needs none"""
     if nbytes < 0:
         _lib.check(-1, name)
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _new(like, shape, contiguous):
+    """an uninitialised tensor of like's type and device; contiguous: `like` is, and has this shape"""
+    return torch.empty_like(like) if contiguous else like.new_empty(shape)
 
 
 def empty(shape, fmt='e4m3', device='cuda'):
@@ -243,7 +259,7 @@ def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=
     d = _lib.MxWgradDesc(dy.data_ptr(), qp, sp, out.data_ptr(), None, p_ld, q_ld, s_ld, _dtype(dy, 'conv_weight_grad'),
                          n, hp, wp, a, hq, wq, b, kh, kw, stride, pad, accumulate)
     ref = C.byref(d)
-    ws = _workspace(_lib.load().msc_mx_wgrad_workspace_bytes(ref), dy, 'msc_mx_wgrad_workspace_bytes')
+    ws = _workspace(_entry('msc_mx_wgrad_workspace_bytes')(ref), dev, 'msc_mx_wgrad_workspace_bytes')
     if ws is not None:
         d.ws = ws.data_ptr()
     _run('msc_mx_wgrad', dev, ref)
@@ -265,7 +281,7 @@ def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=N
     rows, dout_ld = _rows(dout, 'batchnorm_backward')
     _, yp, y_ld, sp, s_ld = saved._args('batchnorm_backward')
     _same_device('batchnorm_backward', dev, saved, relu_mask)
-    dt, dtype = _dtype(dout, 'batchnorm_backward'), dout.dtype
+    dt, dtype, dense = _dtype(dout, 'batchnorm_backward'), dout.dtype, dout.is_contiguous()
     relu, mask_ld = 0, 0
     if relu_mask is not None:
         per = 4 if dt == _lib.F32 else 8
@@ -275,15 +291,15 @@ def batchnorm_backward(dout, saved, gamma, mean, invstd, relu_mask=None, scale=N
     elif scale is not None:
         relu = 2
     if dy is None:
-        dy, dy_ld = torch.empty(dout.shape, dtype=dtype, device=dev), c
+        dy, dy_ld = _new(dout, dout.shape, dense), c
     else:
         dy_ld = _rows(_out(dy, dout.shape, dtype, dev, 'batchnorm_backward'), 'batchnorm_backward')[1]
-    dgamma = torch.empty(c, dtype=torch.float32, device=dev)
-    dbeta = dgamma.new_empty(c)
-    dres = torch.empty(dout.shape, dtype=dtype, device=dev) if residual else None
-    ws = _workspace(_lib.load().msc_mx_bn_bwd_workspace_bytes(rows, c), dout, 'msc_mx_bn_bwd_workspace_bytes')
+    mean_p = _vector(mean, c, dev, 'batchnorm_backward: mean')
+    dgamma, dbeta = _new(mean, (c,), mean.dim() == 1), _new(mean, (c,), mean.dim() == 1)
+    dres = _new(dout, dout.shape, dense) if residual else None
+    ws = _workspace(_entry('msc_mx_bn_bwd_workspace_bytes')(rows, c), dev, 'msc_mx_bn_bwd_workspace_bytes')
     d = _lib.MxBnBwdDesc(dout.data_ptr(), yp, sp, relu_mask.data_ptr() if relu_mask is not None else None,
-                         _vector(gamma, c, dev, 'batchnorm_backward: gamma'), _vector(mean, c, dev, 'batchnorm_backward: mean'),
+                         _vector(gamma, c, dev, 'batchnorm_backward: gamma'), mean_p,
                          _vector(invstd, c, dev, 'batchnorm_backward: invstd'), _vector(scale, c, dev, 'batchnorm_backward: scale'),
                          _vector(shift, c, dev, 'batchnorm_backward: shift'), dgamma.data_ptr(), dbeta.data_ptr(), dy.data_ptr(),
                          dres.data_ptr() if residual else None, ws.data_ptr() if ws is not None else None, dout_ld, y_ld, s_ld, mask_ld, dy_ld, c, rows,
@@ -315,7 +331,7 @@ def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=N
         xp, xcp, xsp, xc_ld, xs_ld = x.data_ptr(), None, None, 0, 0
     shape = x.shape[:-1] + (n,)
     if out is None:
-        out, out_ld = torch.empty(shape, dtype=dtype, device=dev), n
+        out, out_ld = torch.empty(shape, dtype=dtype, device=dev) if packed else x.new_empty(shape), n
     else:
         out_ld = _rows(_out(out, shape, dtype, dev, 'linear'), 'linear')[1]
     _same_device('linear', dev, w)
@@ -327,7 +343,7 @@ def linear(x, w, scale=None, shift=None, res=None, relu=False, dtype=None, out=N
                           out.data_ptr(), None, x_ld, xc_ld, xs_ld, w_ld, ws_ld, res_ld, out_ld, m,
                           _dtype(out, 'linear'), k, n, relu)
     ref = C.byref(d)
-    ws = _workspace(_lib.load().msc_mx_linear_workspace_bytes(ref), w, 'msc_mx_linear_workspace_bytes')
+    ws = _workspace(_entry('msc_mx_linear_workspace_bytes')(ref), dev, 'msc_mx_linear_workspace_bytes')
     if ws is not None:
         d.ws = ws.data_ptr()
     _run('msc_mx_linear', dev, ref)
