@@ -6,7 +6,8 @@
 // Operand roles.  w is the instruction's A operand (rows of the result: n), x its B operand (columns: m): a lane then holds consecutive n of one m, and the
 // fragment rows are dealt out so that its fragments make two runs of eight channels, which move in 16-byte pieces.
 //
-// Three forms: up to 16 (64) rows, the weights streamed once by blocks of 16 channels; a few tiles' channels, x quantised by the tile kernel itself; else packing,
+// Three forms: up to 16 rows (64 of a long reduction, or packed), the weights streamed once by blocks of 16 channels; up to 64 rows of a short one, or a few tiles'
+// channels, x quantised by the tile kernel itself; else packing,
 // then tiles of 256 x 256 (fewer: 128 x 128, 64 x 64).
 //
 // What bounds them.  1 x 4096 -> 4096: 6.1 us on the device for 9 MB, one wave's chain of loads; the call takes 12 us of host time.  8192 x 1024 -> 256: 12 us for
@@ -255,9 +256,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(LinArgs a) {
 // quantised once or a few times.  x comes through registers (a quad of lanes a block, as in packing), w by LDS-DMA.  WM x WN = 4 waves, FM fragments of rows each.
 template <typename T, int WM, int WN, int FM>
 __global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xin, long xin_ld) {
-    constexpr int WAVES = 4, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN, DW = TN / 8 / WAVES, DSW = (TN / 32 + WAVES - 1) / WAVES;
+    constexpr int WAVES = 4, FN = 4, TM = WM * FM * 16, TN = WN * 64, ROWS = TM + TN, DW = TN / 8 / WAVES;
     constexpr int SCALES = ROWS * ROWB, STAGE = SCALES + ROWS * 8, CHUNKS = TM * UNITS * 4 / 256;
-    static_assert(WM * WN == WAVES && 2 * STAGE <= 80 * 1024, "two blocks per CU");
+    static_assert(WM * WN == WAVES && TN <= 256 && 2 * STAGE <= 80 * 1024, "a row of scales per thread, two blocks per CU");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wid / WN, wn = wid % WN, g = lane >> 4, pl = lane & 15;
@@ -266,27 +267,36 @@ __global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xi
     const int n0 = (int)(blockIdx.x % (unsigned)a.tiles_n) * TN;
     const int last_m = (int)min((long)TM, a.M - m0) - 1, last_n = min(TN, a.N - n0) - 1;
     const u32x4_t rw = make_srd(a.w + (long)n0 * a.w_ld, (unsigned)(last_n * a.w_ld + a.nb * 16));
-    const u32x4_t rws = make_srd(a.ws + (long)n0 * a.ws_ld, (unsigned)(last_n * a.ws_ld + (a.nb + 3) / 4 * 4));
     const int u = (lane & 7) ^ ((wid * 8 + (lane >> 3)) >> 1 & 7);
-    unsigned wo[DW], wso[DSW];
+    unsigned wo[DW];
 #pragma unroll
     for (int i = 0; i < DW; ++i) wo[i] = (unsigned)min(lin_channel((i * WAVES + wid) * 8 + (lane >> 3)), last_n) * (unsigned)a.w_ld + u * 16;
-#pragma unroll
-    for (int i = 0; i < DSW; ++i) wso[i] = (unsigned)min(lin_channel(min(i * WAVES + wid, TN / 32 - 1) * 32 + (lane >> 1)), last_n) * (unsigned)a.ws_ld + (lane & 1) * 4;
     auto request = [&](int s, char* st) {
-        const bool live = s * UNITS + u < a.nb, live_s = s * UNITS + (lane & 1) * 4 < a.nb;
+        const bool live = s * UNITS + u < a.nb;
 #pragma unroll
         for (int i = 0; i < DW; ++i) dma16(rw, st + TM * ROWB + (i * WAVES + wid) * 1024, live ? wo[i] + s * ROWB : OOB_OFF, 0);
-#pragma unroll
-        for (int i = 0; i < DSW; ++i) dma4(rws, st + SCALES + TM * 8 + min(i * WAVES + wid, TN / 32 - 1) * 256, live_s ? wso[i] + s * UNITS : OOB_OFF);
     };
     // chunk i of thread t: eight channels, number t % 32 of a step, of row t / 32 + 8 i
     const int xr = tid >> 5, xc = tid & 31;
     Chunk<T> xv[CHUNKS];
+    // w's scales come through registers too, a row per thread: eight bytes at any alignment (odd row pitches need no launch that lays them out)
+    typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1), may_alias));
+    const uint8_t* const wsr = a.ws + (long)(n0 + min(lin_channel(tid), last_n)) * a.ws_ld;
+    uint2 sv = make_uint2(0, 0);
     auto fetch = [&](int s) {
         const int k = s * (UNITS * BLOCK) + xc * 8;
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) xv[i] = load_chunk<T>(xin + (m0 + min(xr + 8 * i, last_m)) * xin_ld + k, a.K - k);
+        const int blocks = a.nb - s * UNITS;
+        const uint8_t* const p = wsr + s * UNITS;
+        if (blocks >= UNITS) {
+            sv = __builtin_bit_cast(uint2, *reinterpret_cast<const u32x2_any*>(p));
+        } else {
+            unsigned e[UNITS];
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) e[i] = p[min(i, blocks - 1)];
+            sv = make_uint2(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24);
+        }
     };
     auto put = [&](char* st) {
 #pragma unroll
@@ -298,6 +308,7 @@ __global__ __launch_bounds__(256, 2) void mx_fused_kernel(LinArgs a, const T* xi
             *reinterpret_cast<unsigned*>(st + r * ROWB + (b ^ ((r >> 1) & 7)) * 16 + (xc & 3) * 4) = encode8_e2m1(q);
             if ((xc & 3) == 0) st[SCALES + r * 8 + b] = (char)e;
         }
+        if (tid < TN) *reinterpret_cast<uint2*>(st + SCALES + (TM + tid) * 8) = sv;
     };
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -425,9 +436,10 @@ template <typename T, int FM, bool FUSED> __global__ __launch_bounds__(FEW_THREA
 
 constexpr int FUSED_ROWS = 16, FEW_ROWS = 64;
 constexpr int64_t FUSED_LDS = 64 * 1024;
-// x quantised by the tile kernel itself (mx_fused_kernel): for weights of at most two waves' channels, and where 512 blocks of 16 (32) x 256 cover the result and the
+// x quantised by the tile kernel itself (mx_fused_kernel): for up to 64 rows of a short reduction, for weights of at most two waves' channels, and where 512 blocks of 16 (32) x 256 cover the result and the
 // reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 12.4 : 17.5; 131072 x 256 -> 64 27.5 : 42.0; 32768 x 512 -> 128 15.7 : 21.9;
 // 2048 x 512 -> 2048 12.7 : 15.3; but 8192 x 1024 -> 1024 31.7 : 26.9, 1024 x 4096 -> 1024 29.5 : 22.4, 8192 x 4096 -> 512 48.4 : 43.2, 131072 x 64 -> 256 58.8 : 38.3
+// and 24 x 1024 -> 4096 8.9 : 8.2, 64 x 1024 -> 1024 8.9 : 10.2, 64 x 256 -> 256 5.2 : 8.6, 64 x 4096 -> 128 40 : 16 (packing, then the kernel for few rows)
 constexpr int FUSED_CHANNELS = 128, FUSED_BLOCKS = 512, FUSED_K = 1024;
 constexpr int64_t FUSED_MOST = 1ll << 29;      // rows: 2^23 blocks, whose 2^31 threads are within a launch; the form behind the packing has a grid of the card's size
 
@@ -437,16 +449,16 @@ LinPlan lin_plan(const msc_mx_linear_desc* d) {
     LinPlan p;
     p.nb = ((int64_t)d->K + BLOCK - 1) / BLOCK;
     p.fused = d->x && d->M <= FUSED_ROWS && few_lds(d->M, p.nb) <= FUSED_LDS;
-    p.few = d->M <= FEW_ROWS;
     const int64_t tiles = (d->M + 15) / 16 * ((d->N + 255) / 256);
     p.tile_rows = tiles <= FUSED_BLOCKS ? 1 : 2;                // fragments of 16
-    p.tile = d->x && !p.few && d->M <= FUSED_MOST && (d->N <= FUSED_CHANNELS || (tiles <= 2 * FUSED_BLOCKS && d->K <= FUSED_K));
+    p.tile = d->x && !p.fused && (d->M <= FEW_ROWS ? d->K <= FUSED_K : d->M <= FUSED_MOST && (d->N <= FUSED_CHANNELS || (tiles <= 2 * FUSED_BLOCKS && d->K <= FUSED_K)));
+    p.few = d->M <= FEW_ROWS && !p.tile;
     p.pack = d->x && !p.fused && !p.tile;
     p.xc_ld = p.nb * E2M1::BYTES;
     p.s_ld = (p.nb + 3) / 4 * 4;                               // rows of scales start on dwords
     p.codes = p.pack ? d->M * p.xc_ld : 0;                     // a multiple of 16
     p.scales = p.pack || !(p.few || p.tile || dword_rows(d->x_scales, d->xs_ld)) ? (d->M * p.s_ld + 15) / 16 * 16 : 0;
-    p.w_scales = p.few || dword_rows(d->w_scales, d->s_ld) ? 0 : (d->N * p.s_ld + 15) / 16 * 16;
+    p.w_scales = p.few || p.tile || dword_rows(d->w_scales, d->s_ld) ? 0 : (d->N * p.s_ld + 15) / 16 * 16;
     p.bytes = p.codes + p.scales + p.w_scales;
     return p;
 }
@@ -481,7 +493,7 @@ template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
     const int64_t tiles = (a.M + TM - 1) / TM * b.tiles_n;
-    if (TN * a.w_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
+    if (TN * a.w_ld >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
     auto k = mx_fused_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -550,11 +562,11 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
         if (rc) return rc;
     }
     auto aligned_rows = [&](const uint8_t*& s, long& ld, int64_t rows, uint8_t* to) {
-        if (p.few || dword_rows(s, ld)) return;
+        if (p.few || p.tile || dword_rows(s, ld)) return;
         hipLaunchKernelGGL(mx_scale_rows_kernel, dim3((unsigned)(rows < 4096 ? (rows + 3) / 4 : 1024)), dim3(256), 0, (hipStream_t)stream, s, ld, to, (long)p.s_ld, (long)rows, (int)p.nb);
         s = to; ld = p.s_ld;
     };
-    if (!p.tile) aligned_rows(a.xs, a.xs_ld, d->M, scales);
+    aligned_rows(a.xs, a.xs_ld, d->M, scales);
     aligned_rows(a.ws, a.ws_ld, d->N, scales + p.scales);
     a.w = d->w; a.w_ld = d->w_ld;
     a.scale = d->scale; a.shift = d->shift; a.res = d->res; a.out = d->out;

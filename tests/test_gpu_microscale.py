@@ -344,6 +344,13 @@ def test_linear(m, k, n, dtype):
     assert torch.equal(buf, mx.linear(x, w, scale=scale, shift=shift, res=res, relu=True))
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('m,k,n', [(17, 1025, 300), (33, 1024, 65), (64, 2050, 33), (64, 1023, 520), (31, 1, 257)])
+def test_linear_of_some_rows(m, k, n, dtype):
+    """17 to 64 rows, of a short reduction (one launch) and a long one; rows of scales off the dword"""
+    test_linear(m, k, n, dtype)
+
+
 @pytest.mark.parametrize('dtype,m,k,n', [('bf16', 2100, 300, 2100), ('fp16', 4113, 72, 4100), ('bf16', 4113, 1100, 4100), ('fp32', 2100, 1100, 2100)])
 def test_linear_tiles(dtype, m, k, n):
     """the large tiles: several per block, ragged in every direction, scale rows off the dword, a lost block of x and of w"""
