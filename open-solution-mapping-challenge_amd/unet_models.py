@@ -1233,6 +1233,7 @@ class _Builder:
 
     def _conv_bn_ckpt_bwd(self, name, x, x8, y, y8, conv, bn, geo, out, res, mean, invstd, rmask):
         net, lib, P, bwd = self.net, self.lib, self.prog, self.prog.bwd
+        self.flush_wgrads()                       # the decoder's, in one launch now: their range of the gradients is final before the encoder begins (trainer.ddp_plan)
         dout = self.grad_of(out)
         d = _lib.MxBnBwdDesc()
         d.dout, d.dout_ld, d.rows, d.C, d.dtype = dout.ptr, dout.ld, out.pixels, conv.out_channels, self.dt

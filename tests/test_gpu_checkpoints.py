@@ -160,3 +160,27 @@ def test_transformer_takes_the_option():
     assert t.model.activation_checkpoint == 'e4m3'
     with pytest.raises(ValueError, match='activation_checkpoint'):
         models.PyTorchUNet(arch, dict(train, activation_checkpoint='fp8'), {})
+
+
+@pytest.mark.parametrize('depth', [34, 101])
+def test_pieces_of_the_backward_leave_final_gradients(depth):
+    """the data-parallel step sends a range of the gradients off as soon as the launches in front of a cut are enqueued: nothing behind the cut may write it again"""
+    from mapping_challenge_amd.trainer import ddp_plan
+    from mapping_challenge_amd.unet_models import _Program
+    net = network(depth, unet_ref.seeded_state_dict(unet_ref.UNetResNetRef(depth)), 'bf16', 'e4m3')
+    x = unet_ref.synthetic_batch(2, 64, 64).cuda()
+    prog = net.train_forward(x)
+    prog.dlogits.copy_(torch.randn(prog.dlogits.shape, generator=torch.Generator().manual_seed(3)) * 1e-2)
+    flat = net.flat_grads
+    plan, kept, beg = ddp_plan(prog, flat, nchunks=4), [], 0
+    assert len(plan) == 4 and sum(hi - lo for _, lo, hi in plan if lo is not None) == flat.numel()
+    assert sum(lo is not None for _, lo, _ in plan) >= 3                   # the encoder's gradients leave in pieces too
+    flat.zero_()
+    prog.stem_dw.zero_()
+    for end, lo, hi in plan:
+        _Program.run_backward(prog.bwd[beg:end], flat.device)
+        beg = end
+        if lo is not None:
+            kept.append((lo, hi, flat[lo:hi].clone()))
+    for lo, hi, then in kept:
+        assert torch.equal(flat[lo:hi], then) and torch.isfinite(then).all()
