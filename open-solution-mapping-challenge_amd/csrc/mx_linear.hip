@@ -10,7 +10,7 @@
 // channels, x quantised by the tile kernel itself; else packing,
 // then tiles of 256 x 256 (fewer: 128 x 128, 64 x 64).
 //
-// What bounds them.  1 x 4096 -> 4096: 6.1 us on the device for 9 MB, one wave's chain of loads; the call takes 12 us of host time.  8192 x 1024 -> 256: 12 us for
+// What bounds them.  1 x 4096 -> 4096: 6.1 us on the device for 9 MB, one wave's chain of loads; the call takes 8.5 us of host time.  8192 x 1024 -> 256: 12 us for
 // 21 MB, the chain of a step (read, quantise, LDS, products) on two blocks per CU.  8192 x 4096 -> 4096 with a residual: 17.5 us of packing, then 113-125 us of
 // product (275 GFLOP: 2.2-2.4 PFLOP/s).  Taken apart, its requests alone take 49 us (1 GB from the L2s at the 10-11 TB/s they deliver), reads and products
 // 45, the epilogue some 40: 134 MB of residual and result, moved by all CUs in step, with no registers left to hold a tile back (256 in use).  Requesting the
