@@ -522,8 +522,11 @@ template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const 
         if (p.tile_rows == 1) return lin_launch_fused<T, 1, 4, 1>(a, d, st);
         return lin_launch_fused<T, 1, 4, 2>(a, d, st);
     }
-    if (tiles(256, 256) >= 256) return lin_launch<T, 2, 4, 8>(a, st);
-    if (tiles(128, 128) >= 256) return lin_launch<T, 2, 2, 4>(a, st);
+    // A larger tile reads less from the caches; a smaller one is taken while all of its tiles are resident at once (two of 128 x 128, four of 64 x 64 to a CU).  us on the
+    // device, large : small: 2048 x 2048 -> 4096 (512 tiles) 30.8 : 23.0, 20480 x 2048 -> 300 (480) 31.2 : 23.6, 2304 x 2048 -> 4096 (576) 31.8 : 33.4, 3328 x 2048 -> 4096 (832) 32.6 : 38.9;
+    // 2048 x 2048 -> 2048 (1024) 17.5 : 15.2, 12288 x 2048 -> 300 (960) 21.8 : 17.2, 2048 x 2048 -> 2560 (1280) 21.2 : 21.8, 1536 x 2048 -> 4096 (1536) 21.7 : 25.3
+    if (tiles(128, 128) > 2 * 256) return lin_launch<T, 2, 4, 8>(a, st);
+    if (tiles(64, 64) > 4 * 256) return lin_launch<T, 2, 2, 4>(a, st);
     return lin_launch<T, 2, 1, 2>(a, st);
 }
 
