@@ -345,14 +345,22 @@ template <int TA, int TB, int SLICES> __global__ __launch_bounds__(THREADS) void
 struct WgPlan { int ta, tb, kg, tiles_a, tiles_b, splits, chunk; };
 WgPlan wg_plan(const msc_mx_wgrad_desc* d) {
     WgPlan p;
-    p.ta = d->A > 64 ? 128 : 64;
-    p.tb = d->B > 64 ? 128 : 64;
+    const int64_t M = (int64_t)d->N * d->Hp * d->Wp, taps = d->KH * d->KW;
+    const int kp = d->dtype == MSC_F32 ? 32 : 64;
+    // Tiles of 128 read less, but are few and take longer to start.  They are for 2^31 products and more where their blocks can fill the card: without splitting the pixels, or with
+    // ranges that stay long.  us with the join, 128 : 64, bf16: 8192 pixels, 256 x 256, 3x3 29.8 : 50.3; 6144 27.8 : 39.3; 2048 22.5 : 17.9; 131072, 256 x 64 20.5 : 21.0;
+    // 65536, 256 x 64 17.2 : 15.8; 32768, 256 x 256 21.3 : 22.9; 400, 384 x 384, 3x3 19.3 : 12.5; 4096, 128 x 512 13.6 : 11.1; 2048 pixels: 512 x 2048 22.6 : 18.4, 1024 x 2048
+    // 30.3 : 25.7, 2048 x 2048 (256 blocks) 42.6 : 47.9, 512 x 512, 3x3 (144 blocks) 39.6 : 36.7
+    const int64_t large = (int64_t)((d->A + 127) / 128) * ((d->B + 127) / 128) * taps;
+    const bool wide = M * taps * d->A >= ((1ll << 31) + d->B - 1) / d->B && (large >= 160 || (large <= 128 && M >= 4096));
+    p.ta = wide && d->A > 64 ? 128 : 64;
+    p.tb = wide && d->B > 64 ? 128 : 64;
     p.tiles_a = (d->A + p.ta - 1) / p.ta;
     p.tiles_b = (d->B + p.tb - 1) / p.tb;
-    const int64_t M = (int64_t)d->N * d->Hp * d->Wp, all = (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW;
-    const int kp = d->dtype == MSC_F32 ? 32 : 64;
-        // two groups of waves to a block and one block to a CU where every group has four steps to do: half the partial sums of two blocks with one group each
-    // (3x3 above: 24.1 + 5.4 us to join, against 24.8 + 7.2; 1x1: 16.7 + 4.0 against 17.3 + 4.5).  Fewer pixels: more, smaller blocks
+    const int64_t all = (int64_t)p.tiles_a * p.tiles_b * taps;
+    // two groups of waves to a block and one block to a CU where every group has four steps to do: half the partial sums of two blocks with one group each
+    // (3x3 above: 24.1 + 5.4 us to join, against 24.8 + 7.2; 1x1: 16.7 + 4.0 against 17.3 + 4.5).  Tiles of 128 always have: 2^31 products are four
+    // steps for 512 groups.  Less work: more, smaller blocks
     p.kg = M * all >= 256ll * 2 * 4 * kp ? 2 : 1;
     int64_t splits = 512 / p.kg / all, most = (M + 4 * p.kg * kp - 1) / (4 * p.kg * kp);
     if (splits > most) splits = most;
@@ -391,7 +399,9 @@ template <typename T, int TA, int TB, int KG> int wg_launch_tiles(const WgArgs& 
     return MSC_OK;
 }
 template <typename T, int TA, int TB> int wg_launch(const WgPlan& p, const WgArgs& a, bool vec, hipStream_t st) {
-    const int rc = p.kg == 2 ? wg_launch_tiles<T, TA, TB, 2>(a, vec, st) : wg_launch_tiles<T, TA, TB, 1>(a, vec, st);
+    int rc;
+    if constexpr (TA == 64 && TB == 64) rc = p.kg == 2 ? wg_launch_tiles<T, 64, 64, 2>(a, vec, st) : wg_launch_tiles<T, 64, 64, 1>(a, vec, st);
+    else rc = wg_launch_tiles<T, TA, TB, 2>(a, vec, st);
     if (rc || a.splits == 1) return rc;
     const int64_t places = (int64_t)a.tiles * a.taps * TA * TB / 4;
     // enough threads to have the partial sums' reads in flight (256 ranges of 256 x 64: 12.7 us with one slice, 4.5 with sixteen)
@@ -430,9 +440,9 @@ extern "C" int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: q needs 16-byte aligned rows of whole E4M3 blocks and one scale byte per block");
     const WgPlan p = wg_plan(d);
     if (p.splits > 1 && (!d->ws || (uintptr_t)d->ws & 15)) return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: workspace missing or not 16-byte aligned");
-    if ((int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * (p.ta / 32) * (p.tb / 32) >= 1ll << 30 ||
-        (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW * p.splits >= 1ll << 30)
-        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 tiles or more");
+    const int64_t all = (int64_t)p.tiles_a * p.tiles_b * d->KH * d->KW;        // a launch has fewer than 2^32 threads: of the products, of the join
+    if (all * p.splits >= 1ll << 23 || (p.splits > 1 && all * (p.ta / 32) * (p.tb / 32) >= 1ll << 24))
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^23 tiles or more");
     const int64_t hw = (int64_t)d->Hp * d->Wp, image = (int64_t)d->Hq * d->Wq * (d->q_ld > d->s_ld ? d->q_ld : d->s_ld);
     if (((p.chunk - 1) / hw + 2) * image >= 1ll << 31)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: the images of %d output pixels span 2 GiB", p.chunk);

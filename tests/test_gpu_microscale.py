@@ -169,6 +169,14 @@ def test_weight_gradient_of_many_pixels(n, h, w, a, b, k, stride, dtype):
             assert float((got[:, i, j] - ref).norm() / ref.norm()) < 2e-6
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('n,h,w,a,b,k,stride', [(16, 40, 44, 130, 70, 3, 1), (16, 40, 44, 131, 70, 3, 1), (32, 64, 64, 256, 64, 1, 1), (22, 50, 40, 64, 130, 3, 2),
+                                                (2500, 3, 2, 128, 128, 3, 1), (8, 16, 16, 1700, 1701, 1, 1)])
+def test_weight_gradient_of_much_work(n, h, w, a, b, k, stride, dtype):
+    """2^31 products and more: the tiles of 128"""
+    test_weight_gradient_of_many_pixels(n, h, w, a, b, k, stride, dtype)
+
+
 def test_weight_gradient_accumulates_slices_and_repeats():
     from mapping_challenge_amd import microscale as mx
     saved, x = packed((2, 16, 16, 64), 'e4m3', 15)
