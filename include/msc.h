@@ -511,7 +511,8 @@ int msc_mx_unpack(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales,
 
 /* msc_conv_wgrad with q (the layer's input) held in E4M3:  dw[a][kh][kw][b] (+)= sum_m p[m][a] * q[(y*stride-pad+kh, x*stride-pad+kw)][b], fp32.
  * The pixel dimension is split over blocks; the partial sums go to `ws` (msc_mx_wgrad_workspace_bytes(d) bytes, may be 0; 16-byte aligned) and are added
- * in a fixed order.  Any A, B; KH, KW <= 16; p_ld in elements, q_ld / s_ld in bytes.  q's values are exact in every `dtype` they were packed from. */
+ * in a fixed order.  Any A, B; KH, KW <= 16; p_ld in elements, q_ld / s_ld in bytes.  The products are of `dtype`: q's values are exact in the one they were packed
+ * from and in f32; in fp16 what was packed from a wider type loses what fp16 does not hold (past 65504: infinity; below 2^-24: zero) -- take p to f32 there. */
 typedef struct msc_mx_wgrad_desc {
     const void* p;
     const uint8_t* q;

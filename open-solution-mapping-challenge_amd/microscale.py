@@ -26,12 +26,16 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 
 class MxTensor:
     """A packed tensor of shape [..., channels]: codes uint8 [..., blocks * 32 (E4M3) or 16 (E2M1)], scales uint8 [..., blocks], blocks = ceil(channels / 32).
-    Rows of codes start on 16 bytes; both may be slices of wider buffers."""
-    __slots__ = ('_codes', '_scales', '_buf', '_lead', 'channels', 'fmt')
+    Rows of codes start on 16 bytes; both may be slices of wider buffers.
+    dtype: the type of the tensor that was packed (pack sets it), or None where the codes come from elsewhere and nobody said.  The values depend on codes and scales alone; the
+    type says which numbers they can be (conv_weight_grad)."""
+    __slots__ = ('_codes', '_scales', '_buf', '_lead', 'channels', 'fmt', 'dtype')
 
-    def __init__(self, codes, scales, channels, fmt='e4m3'):
+    def __init__(self, codes, scales, channels, fmt='e4m3', dtype=None):
         if fmt not in FORMATS:
             raise ValueError("format must be 'e4m3' or 'e2m1', got %r" % (fmt,))
+        if dtype is not None and dtype not in _DTYPES:
+            raise TypeError('a packed tensor was float32, bfloat16 or float16, got %s' % (dtype,))
         nb = (channels + 31) // 32
         if channels <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise ValueError('a packed tensor has at least one channel, and uint8 codes and scales')
@@ -41,13 +45,13 @@ class MxTensor:
                              % (channels, fmt, nb * FORMATS[fmt][1], nb, tuple(codes.shape), tuple(scales.shape)))
         if codes.device != scales.device:
             raise ValueError('codes and scales are on different devices')
-        self._codes, self._scales, self._buf, self._lead, self.channels, self.fmt = codes, scales, None, lead, channels, fmt
+        self._codes, self._scales, self._buf, self._lead, self.channels, self.fmt, self.dtype = codes, scales, None, lead, channels, fmt, dtype
 
     @classmethod
-    def _made(cls, buf, lead, channels, fmt):
+    def _made(cls, buf, lead, channels, fmt, dtype=None):
         """over one allocation, the codes and then the scales; the two tensors are made when somebody asks for them (each costs the host what a launch does)"""
         t = cls.__new__(cls)
-        t._codes, t._scales, t._buf, t._lead, t.channels, t.fmt = None, None, buf, lead, channels, fmt
+        t._codes, t._scales, t._buf, t._lead, t.channels, t.fmt, t.dtype = None, None, buf, lead, channels, fmt, dtype
         return t
 
     def _split(self):
@@ -211,6 +215,7 @@ def pack(x, fmt='e4m3', out=None):
         _same_device('pack', dev, out)
         _, cp, c_ld, sp, s_ld = out._args('pack')
     _run('msc_mx_pack', dev, x.data_ptr(), ld, _dtype(x, 'pack'), cp, c_ld, sp, s_ld, fid, rows, c)
+    out.dtype = x.dtype
     return out
 
 
@@ -230,12 +235,16 @@ def unpack(t, dtype=torch.bfloat16, out=None):
 def conv_weight_grad(dy, saved, kernel=1, stride=1, pad=0, out=None, accumulate=False):
     """float32 [A, KH, KW, B]: the weight gradient of a convolution whose output gradient is dy [N, H, W, A] and whose input [N, Hi, Wi, B] was kept as the E4M3
     MxTensor `saved`.  kernel: a size or (KH, KW).  A linear layer: kernel 1, dy [..., A] and saved [..., B] with the same leading shape.
-    accumulate: added to `out` (which then has to be given) instead of written over it."""
+    accumulate: added to `out` (which then has to be given) instead of written over it.
+    The products are of dy's type, in which every value of a checkpoint of that type is exact.  float16 does not hold every value of a wider one (past 65504, below 2^-24): a
+    float16 dy with a checkpoint that was packed from float32 or bfloat16 (saved.dtype) is turned to float32 first.  saved.dtype None: taken to be dy's."""
     if saved.fmt != 'e4m3':
         raise ValueError('conv_weight_grad: the checkpoint has to be in e4m3, got %s' % saved.fmt)
     if accumulate and out is None:
         raise ValueError('conv_weight_grad: accumulate needs out')
     kh, kw = (kernel, kernel) if isinstance(kernel, int) else kernel
+    if dy.dtype == torch.float16 and saved.dtype not in (None, torch.float16):
+        dy = dy.float()
     rows, p_ld = _rows(dy, 'conv_weight_grad')
     _, qp, q_ld, sp, s_ld = saved._args('conv_weight_grad')
     a, b = dy.shape[-1], saved.channels
