@@ -493,8 +493,8 @@ int msc_size_matrix(const int32_t* labels, int32_t* sizes, int32_t* areas, int B
  *   codes  : MSC_MX_E4M3 one byte per element; MSC_MX_E2M1 two elements per byte, the even channel in the low nibble.  The last block of a row is
  *            zero-filled up to MSC_MX_BLOCK, so a row takes nb*32 (nb*16) bytes, nb = ceil(C/32); codes_ld bytes from row to row, a multiple of 16,
  *            base 16-byte aligned.
- *   scales : one byte per block, nb bytes per row, scales_ld bytes from row to row.  Byte e (1 .. 254) stands for 2^(e-127), 255 for NaN.
- *   value  : code * 2^(e-127).
+ *   scales : one byte per block, nb bytes per row, scales_ld bytes from row to row.  Byte e (0 .. 254) stands for 2^(e-127), 255 for NaN.
+ *   value  : code * 2^(e-127).  (Codes from elsewhere may have bytes below 10, which packing does not write; a 16-bit result or product rounds such values to its denormals.)
  * Packing takes the smallest power of two under which no element passes the largest code (448 / 6) and rounds to the nearest code, ties to even
  * (an error of at most 2^-4 / 2^-2 of the value, or half the smallest code times the scale).  Elements whose code would stand for a value past the
  * largest finite one of `dtype` are clamped first (fp16 61440 / 49152, bf16 and f32 1.875 / 1.5 * 2^127).  The scale's byte is at least 10, so that every

@@ -29,8 +29,8 @@ template <typename F> __device__ __forceinline__ unsigned scale_field(unsigned a
     return (unsigned)max(e, MIN_E);                                   // at most 255 - 2 + 1 = 254
 }
 __device__ __forceinline__ float pow2_field(unsigned e) { return __uint_as_float(e << 23); }
-// 2^(e - 127) of a stored scale byte; NaN for 255.  (Field 0, 2^-127, is below what packing writes: it reads as zero, like a flushed denormal.)
-__device__ __forceinline__ float scale_value(unsigned e) { return e == NAN_E ? __uint_as_float(0x7fc00000u) : pow2_field(e); }
+// 2^(e - 127) of a stored scale byte; NaN for 255.  Byte 0 is 2^-127, a denormal float whose one bit lies below the exponent field
+__device__ __forceinline__ float scale_value(unsigned e) { return e == NAN_E ? __uint_as_float(0x7fc00000u) : __uint_as_float(max(e << 23, 0x400000u)); }
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // 8 elements in units of the scale -> codes

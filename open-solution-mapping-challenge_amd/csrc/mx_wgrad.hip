@@ -63,7 +63,7 @@ template <typename T, int UPR> __device__ __forceinline__ void stage_q(char* row
         w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
         e = 127;
     }
-    const float s = pow2_field(max(e, 1u));                            // 0: a pixel that was not read
+    const float s = scale_value(e);                                    // (a pixel that was not read: codes and byte 0)
     const unsigned c[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 2) {
         unsigned o[8];
