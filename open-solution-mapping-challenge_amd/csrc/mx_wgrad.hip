@@ -381,9 +381,9 @@ int wg_check(const msc_mx_wgrad_desc* d) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: bad shape");
     if (d->KH <= 0 || d->KW <= 0 || d->KH > 16 || d->KW > 16 || d->stride <= 0 || d->stride > 16 || d->pad < 0 || d->pad > 16)
         return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: kernel %dx%d, stride %d, padding %d", d->KH, d->KW, d->stride, d->pad);
-    if ((int64_t)d->N * d->Hp * d->Wp >= 1ll << 30 || (int64_t)d->Hq * d->Wq >= 1ll << 30)
-        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 pixels or more");
-    if ((int64_t)d->Hq * d->Wq * d->q_ld >= 1ll << 28 || (int64_t)d->Hq * d->Wq * d->s_ld >= 1ll << 28 || d->p_ld >= 1ll << 24)
+    const int64_t hw = (int64_t)d->Hp * d->Wp, image = (int64_t)d->Hq * d->Wq, most = 1ll << 28;      // (factors first: no product below passes 64 bits)
+    if (hw >= 1ll << 30 || d->N * hw >= 1ll << 30 || image >= 1ll << 30) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: 2^30 pixels or more");
+    if (d->q_ld >= most || d->s_ld >= most || image * d->q_ld >= most || image * d->s_ld >= most || d->p_ld >= 1ll << 24)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: an image of 2^28 bytes of codes or more, or rows of 2^24 elements");
     return MSC_OK;
 }

@@ -1,8 +1,11 @@
 """CPU: refusals of the microscaled operators at the limits of their arguments.  No kernel is launched."""
+import ctypes as C
+
 import pytest
 import torch
 
-from mapping_challenge_amd import microscale as mx
+from mapping_challenge_amd import _lib, microscale as mx
+from test_microscale import refused, wgrad_desc
 
 
 def test_packed_tensor_of_an_unknown_type_is_refused():
@@ -11,3 +14,12 @@ def test_packed_tensor_of_an_unknown_type_is_refused():
     assert mx.MxTensor(codes, scales, 40, dtype=torch.bfloat16).dtype == torch.bfloat16
     with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
         mx.MxTensor(codes, scales, 40, dtype=torch.float64)
+
+
+def test_weight_gradient_sizes_whose_products_pass_64_bits():
+    """2^22 * 2^21 * 2^21 pixels are 0 modulo 2^64: the plan divided by it, and the process ended"""
+    lib = _lib.load()
+    for bad, word in ((dict(N=1 << 22, Hp=1 << 21, Wp=1 << 21), '2^30'), (dict(Hp=1 << 30, Wp=1 << 30), '2^30'), (dict(Hq=1 << 30, Wq=1 << 30, q_ld=32), '2^30'),
+                      (dict(Hq=2, Wq=2, q_ld=1 << 62), '2^28'), (dict(Hq=2, Wq=2, s_ld=1 << 62), '2^28'), (dict(Hq=1 << 14, Wq=1 << 14, q_ld=1 << 36), '2^28')):
+        assert lib.msc_mx_wgrad_workspace_bytes(C.byref(wgrad_desc(**bad))) == -1
+        refused(lib.msc_mx_wgrad(C.byref(wgrad_desc(**bad)), None), word)
