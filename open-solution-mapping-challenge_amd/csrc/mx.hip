@@ -406,6 +406,7 @@ template <typename T, int RELU> __global__ __launch_bounds__(BN_FEW_THREADS) voi
         if (rg + k * BN_FEW_GROUPS < a.rows) bn_store<T, RELU>(a, rg + k * BN_FEW_GROUPS, c0, left, raw[k], f, mean, sc, sh);
 }
 
+constexpr int64_t BN_ROWS_END = 1ll << 40;         // past any memory; the plan's sums stay far from 64 bits
 struct BnPlan { int cols_log2, ctiles, strips, apply_strips; };
 BnPlan bn_plan(int64_t rows, int C) {
     BnPlan p;
@@ -442,14 +443,14 @@ template <typename T> void bn_by_relu(int relu, const BnArgs& a, const BnPlan& p
 }  // namespace
 
 extern "C" int64_t msc_mx_bn_bwd_workspace_bytes(int64_t rows, int C) {
-    if (rows <= BN_FEW || C <= 0 || C > (1 << 24)) return 0;
+    if (rows <= BN_FEW || rows >= BN_ROWS_END || C <= 0 || C > (1 << 24)) return 0;
     return (int64_t)C * 16 * (1 + bn_plan(rows, C).strips);
 }
 
 extern "C" int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream) {
     if (!d) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: null descriptor");
     if (!msc_dtype_ok(d->dtype)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: unknown dtype %d", d->dtype);
-    if (d->rows <= 0 || d->C <= 0 || d->C > (1 << 24))
+    if (d->rows <= 0 || d->rows >= BN_ROWS_END || d->C <= 0 || d->C > (1 << 24))
         return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: bad shape (%lld rows, %d channels)", (long long)d->rows, d->C);
     if (!d->dout || !d->dy || !d->mean || !d->invstd || (!d->ws && d->rows > BN_FEW)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: null pointer");
     if (d->relu != 0 && d->relu != 2 && d->relu != 3) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: relu is 0, 2 or 3, got %d", d->relu);
