@@ -471,15 +471,38 @@ int lin_check(const msc_mx_linear_desc* d) {
     return MSC_OK;
 }
 
+// rows and channels of a block's tile (the kernels' TM, TN); 0: the form for few rows, which has none
+struct LinTile { int m, n; };
+LinTile lin_tile(const LinPlan& p, int64_t M, int64_t N) {
+    if (p.few) return {0, 0};
+    if (p.tile) {
+        if (N <= 64) return {64, 64};
+        if (N <= 128) return {64, 128};
+        return {p.tile_rows * 16, 256};
+    }
+    auto tiles = [&](int t) { return (M + t - 1) / t * ((N + t - 1) / t); };
+    // A larger tile reads less from the caches; a smaller one is taken while all of its tiles are resident at once (two of 128 x 128, four of 64 x 64 to a CU).  us on the
+    // device, large : small: 2048 x 2048 -> 4096 (512 tiles) 30.8 : 23.0, 20480 x 2048 -> 300 (480) 31.2 : 23.6, 2304 x 2048 -> 4096 (576) 31.8 : 33.4, 3328 x 2048 -> 4096 (832) 32.6 : 38.9;
+    // 2048 x 2048 -> 2048 (1024) 17.5 : 15.2, 12288 x 2048 -> 300 (960) 21.8 : 17.2, 2048 x 2048 -> 2560 (1280) 21.2 : 21.8, 1536 x 2048 -> 4096 (1536) 21.7 : 25.3
+    const int t = tiles(128) > 2 * 256 ? 256 : tiles(64) > 4 * 256 ? 128 : 64;
+    return {t, t};
+}
+// what a tile's descriptors and the grid can hold
+int lin_tile_check(const LinTile& t, const LinPlan& p, const LinArgs& a) {
+    if (!t.m) return MSC_OK;
+    auto spans = [](int rows, int64_t ld) { return ld >= (1ll << 31) / rows; };
+    if (!p.tile && (a.M + t.m - 1) / t.m * ((a.N + t.n - 1) / t.n) >= 1ll << 30) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^30 tiles or more");
+    if (spans(t.n, a.w_ld) || (!p.tile && (spans(t.m, a.x_ld) || spans(t.m, a.xs_ld) || spans(t.n, a.ws_ld))))
+        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
+    return MSC_OK;
+}
+
 template <typename T, int WM, int WN, int FM> int lin_launch(const LinArgs& a, hipStream_t st) {
     constexpr int TM = WM * FM * 16, TN = WN * 64, LDS = 2 * (TM + TN) * (ROWB + UNITS), RESIDENT = 256 * (LDS > 80 * 1024 ? 1 : LDS > 40 * 1024 ? 2 : 4);
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
     const int64_t tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * b.tiles_n;
     b.tiles_m = (int)tiles_m;
-    if (tiles >= 1ll << 30) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: 2^30 tiles or more");
-    if (TM * a.x_ld >= 1ll << 31 || TN * a.w_ld >= 1ll << 31 || TM * a.xs_ld >= 1ll << 31 || TN * a.ws_ld >= 1ll << 31)
-        return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
     auto k = mx_gemm_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -493,7 +516,6 @@ template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs
     LinArgs b = a;
     b.tiles_n = (a.N + TN - 1) / TN;
     const int64_t tiles = (a.M + TM - 1) / TM * b.tiles_n;
-    if (TN * a.w_ld >= 1ll << 31) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_linear: a tile's rows span 2 GiB");
     auto k = mx_fused_kernel<T, WM, WN, FM>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -502,7 +524,7 @@ template <typename T, int WM, int WN, int FM> int lin_launch_fused(const LinArgs
     hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), LDS, st, b, (const T*)d->x, (long)d->x_ld);
     return MSC_OK;
 }
-template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const msc_mx_linear_desc* d, hipStream_t st) {
+template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const LinTile& t, const msc_mx_linear_desc* d, hipStream_t st) {
     const dim3 few((unsigned)((a.N + 15) / 16));
     const long none = 0;
     if (p.fused) {
@@ -515,18 +537,14 @@ template <typename T> int lin_by_tile(const LinArgs& a, const LinPlan& p, const 
         hipLaunchKernelGGL(k, few, dim3(FEW_THREADS), (size_t)fm * FEW_WAVES * 64 * 16, st, a, (const T*)nullptr, none);
         return MSC_OK;
     }
-    auto tiles = [&](int tm, int tn) { return (a.M + tm - 1) / tm * ((a.N + tn - 1) / tn); };
     if (p.tile) {
-        if (a.N <= 64) return lin_launch_fused<T, 4, 1, 1>(a, d, st);
-        if (a.N <= 128) return lin_launch_fused<T, 2, 2, 2>(a, d, st);
-        if (p.tile_rows == 1) return lin_launch_fused<T, 1, 4, 1>(a, d, st);
+        if (t.n == 64) return lin_launch_fused<T, 4, 1, 1>(a, d, st);
+        if (t.n == 128) return lin_launch_fused<T, 2, 2, 2>(a, d, st);
+        if (t.m == 16) return lin_launch_fused<T, 1, 4, 1>(a, d, st);
         return lin_launch_fused<T, 1, 4, 2>(a, d, st);
     }
-    // A larger tile reads less from the caches; a smaller one is taken while all of its tiles are resident at once (two of 128 x 128, four of 64 x 64 to a CU).  us on the
-    // device, large : small: 2048 x 2048 -> 4096 (512 tiles) 30.8 : 23.0, 20480 x 2048 -> 300 (480) 31.2 : 23.6, 2304 x 2048 -> 4096 (576) 31.8 : 33.4, 3328 x 2048 -> 4096 (832) 32.6 : 38.9;
-    // 2048 x 2048 -> 2048 (1024) 17.5 : 15.2, 12288 x 2048 -> 300 (960) 21.8 : 17.2, 2048 x 2048 -> 2560 (1280) 21.2 : 21.8, 1536 x 2048 -> 4096 (1536) 21.7 : 25.3
-    if (tiles(128, 128) > 2 * 256) return lin_launch<T, 2, 4, 8>(a, st);
-    if (tiles(64, 64) > 4 * 256) return lin_launch<T, 2, 2, 4>(a, st);
+    if (t.m == 256) return lin_launch<T, 2, 4, 8>(a, st);
+    if (t.m == 128) return lin_launch<T, 2, 2, 4>(a, st);
     return lin_launch<T, 2, 1, 2>(a, st);
 }
 
@@ -557,24 +575,27 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
     LinArgs a;
     uint8_t* codes = (uint8_t*)d->ws;
     uint8_t* scales = codes + p.codes;
+    uint8_t* w_scales = scales + p.scales;
     a.x = d->x_codes; a.x_ld = d->xc_ld; a.xs = d->x_scales; a.xs_ld = d->xs_ld;
-    a.ws = d->w_scales; a.ws_ld = d->s_ld;
+    a.w = d->w; a.w_ld = d->w_ld; a.ws = d->w_scales; a.ws_ld = d->s_ld;
+    if (p.pack) { a.x = codes; a.x_ld = p.xc_ld; }
+    if (p.scales) { a.xs = scales; a.xs_ld = p.s_ld; }
+    if (p.w_scales) { a.ws = w_scales; a.ws_ld = p.s_ld; }
+    a.scale = d->scale; a.shift = d->shift; a.res = d->res; a.out = d->out;
+    a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_m = a.tiles_n = 0;
+    const LinTile t = lin_tile(p, d->M, d->N);
+    rc = lin_tile_check(t, p, a);
+    if (rc) return rc;                                         // nothing has been launched so far
     if (p.pack) {
-        a.x = codes; a.x_ld = p.xc_ld; a.xs = scales; a.xs_ld = p.s_ld;
         rc = msc_mx_pack(d->x, d->x_ld, d->dtype, codes, p.xc_ld, scales, p.s_ld, MSC_MX_E2M1, d->M, d->K, stream);
         if (rc) return rc;
     }
-    auto aligned_rows = [&](const uint8_t*& s, long& ld, int64_t rows, uint8_t* to) {
-        if (p.few || p.tile || dword_rows(s, ld)) return;
+    auto aligned_rows = [&](const uint8_t* s, long ld, int64_t rows, uint8_t* to) {
         hipLaunchKernelGGL(mx_scale_rows_kernel, dim3((unsigned)(rows < 4096 ? (rows + 3) / 4 : 1024)), dim3(256), 0, (hipStream_t)stream, s, ld, to, (long)p.s_ld, (long)rows, (int)p.nb);
-        s = to; ld = p.s_ld;
     };
-    aligned_rows(a.xs, a.xs_ld, d->M, scales);
-    aligned_rows(a.ws, a.ws_ld, d->N, scales + p.scales);
-    a.w = d->w; a.w_ld = d->w_ld;
-    a.scale = d->scale; a.shift = d->shift; a.res = d->res; a.out = d->out;
-    a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_m = a.tiles_n = 0;
+    if (p.scales && !p.pack) aligned_rows(d->x_scales, d->xs_ld, d->M, scales);
+    if (p.w_scales) aligned_rows(d->w_scales, d->s_ld, d->N, w_scales);
     hipStream_t st = (hipStream_t)stream;
-    rc = d->dtype == MSC_F32 ? lin_by_tile<float>(a, p, d, st) : d->dtype == MSC_BF16 ? lin_by_tile<bf16_t>(a, p, d, st) : lin_by_tile<f16_t>(a, p, d, st);
+    rc = d->dtype == MSC_F32 ? lin_by_tile<float>(a, p, t, d, st) : d->dtype == MSC_BF16 ? lin_by_tile<bf16_t>(a, p, t, d, st) : lin_by_tile<f16_t>(a, p, t, d, st);
     return rc ? rc : msc_check_launch("msc_mx_linear");
 }

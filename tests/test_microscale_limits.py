@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from mapping_challenge_amd import _lib, microscale as mx
-from test_microscale import bn_desc, refused, wgrad_desc
+from test_microscale import A16, bn_desc, linear_desc, refused, wgrad_desc
 
 
 def test_packed_tensor_of_an_unknown_type_is_refused():
@@ -31,3 +31,19 @@ def test_batchnorm_of_more_rows_than_any_memory():
         assert lib.msc_mx_bn_bwd_workspace_bytes(rows, 64) == 0
         refused(lib.msc_mx_bn_bwd(C.byref(bn_desc(rows=rows)), None), 'shape')
     assert lib.msc_mx_bn_bwd_workspace_bytes((1 << 40) - 1, 64) > 0
+
+
+def test_linear_refuses_before_it_launches():
+    """too many tiles, and rows too far apart for a tile's descriptor: found before x is packed or a row of scales copied (here, without a device, a launch is an error of its own)"""
+    lib = _lib.load()
+    run = lambda **kw: lib.msc_mx_linear(C.byref(linear_desc(**kw)), None)  # noqa: E731
+    refused(run(M=1 << 35, N=2048, out_ld=2048), '2^30')                   # x to be packed
+    many = dict(x=None, x_codes=A16, x_scales=A16 + 1, xc_ld=32, xs_ld=3, M=1 << 35, N=2048, out_ld=2048, w_scales=A16 + 1, s_ld=3)
+    refused(run(**many), '2^30')                                           # scales to be laid out
+    refused(run(M=2000, K=2048, N=3000, out_ld=3000, x_ld=2048, s_ld=64, w_ld=1 << 24), '2 GiB')
+    refused(run(M=200, K=2048, N=300, out_ld=300, x_ld=2048, s_ld=64, w_ld=1 << 62), '2 GiB')
+    refused(run(M=200, w_ld=1 << 25, N=64, out_ld=64), '2 GiB')            # x quantised by the product's own launch
+    far = dict(x=None, x_codes=A16, x_scales=A16, xc_ld=32, xs_ld=2, M=2000, K=2048, N=3000, out_ld=3000, w_ld=1024, s_ld=64, w_scales=A16 + 1)
+    refused(run(**dict(far, xc_ld=1 << 24, xs_ld=64)), '2 GiB')
+    refused(run(**dict(far, xc_ld=1024, xs_ld=1 << 24)), '2 GiB')
+    refused(run(**dict(far, xc_ld=1024, xs_ld=64, w_scales=A16, s_ld=1 << 24)), '2 GiB')
