@@ -499,6 +499,7 @@ int msc_size_matrix(const int32_t* labels, int32_t* sizes, int32_t* areas, int B
  * (an error of at most 2^-4 / 2^-2 of the value, or half the smallest code times the scale).  Elements whose code would stand for a value past the
  * largest finite one of `dtype` are clamped first (fp16 61440 / 49152, bf16 and f32 1.875 / 1.5 * 2^127).  The scale's byte is at least 10, so that every
  * value is a normal bf16 number: magnitudes below 2^-127 (2^-119 for E2M1) become zero.  A block that holds an infinity or NaN stands for 32 NaNs.
+ * Results may not share memory with operands, but for the in-place forms named below; channel slices of one buffer that hold other channels do not.
  * Everything below runs on `stream`, allocates nothing, synchronises nothing and may be captured; outputs are the same bits from run to run. */
 #define MSC_MX_BLOCK 32
 #define MSC_MX_E4M3 0

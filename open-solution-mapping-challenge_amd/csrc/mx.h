@@ -157,6 +157,20 @@ static inline bool packed_ok(const void* codes, int64_t ld, const void* scales, 
     const int64_t nb = ((int64_t)C + BLOCK - 1) / BLOCK;
     return codes && scales && ((uintptr_t)codes & 15) == 0 && ld % 16 == 0 && ld >= nb * block_bytes && s_ld >= nb;
 }
+// Rows of `len` bytes, `pitch` bytes apart.  Two such sets of one pitch (channel slices of one buffer) share a byte where their columns do; of two pitches
+// they are taken to share one as soon as the memory they span does.  Kernels write results while other blocks still read operands, so nothing but the in-place forms
+// that a descriptor names may meet.
+struct Rows { const void* p; int64_t pitch, len, rows; };
+static inline bool meet(const Rows& a, const Rows& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+    const __int128 a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p, a1 = a0 + (__int128)(a.rows - 1) * a.pitch + a.len, b1 = b0 + (__int128)(b.rows - 1) * b.pitch + b.len;
+    if (a1 <= b0 || b1 <= a0) return false;
+    const int64_t pitch = a.rows == 1 ? b.pitch : a.pitch;
+    if ((a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) || (a.rows == 1 && b.rows == 1)) return true;
+    const int64_t off = (int64_t)(((b0 - a0) % pitch + pitch) % pitch);
+    return off < a.len || off + b.len > pitch;
+}
+static inline Rows one_row(const void* p, int64_t len) { return {p, len, len, 1}; }
 static inline bool vec_ok(const void* p, int64_t ld, int dtype) { return ((uintptr_t)p & 15) == 0 && ld % msc_dtype_vec(dtype) == 0; }
 
 }  // namespace mx

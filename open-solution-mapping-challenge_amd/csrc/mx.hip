@@ -95,6 +95,11 @@ int mx_check(const char* name, const void* x, int64_t x_ld, int dtype, const voi
     if (!packed_ok(codes, codes_ld, scales, scales_ld, C, fmt == MSC_MX_E4M3 ? E4M3::BYTES : E2M1::BYTES))
         return msc_fail(MSC_ERR_ARG, "%s: codes need 16-byte aligned rows of whole blocks, scales one byte per block (row pitches %lld / %lld, %d channels)", name,
                         (long long)codes_ld, (long long)scales_ld, C);
+    const int es = msc_dtype_size(dtype);
+    const int64_t nb = ((int64_t)C + BLOCK - 1) / BLOCK;
+    const Rows t{x, x_ld * es, (int64_t)C * es, rows};
+    if (meet(t, {codes, codes_ld, nb * (fmt == MSC_MX_E4M3 ? E4M3::BYTES : E2M1::BYTES), rows}) || meet(t, {scales, scales_ld, nb, rows}))
+        return msc_fail(MSC_ERR_ARG, "%s: the tensor shares memory with its codes or scales", name);
     return MSC_OK;
 }
 
@@ -468,6 +473,14 @@ extern "C" int msc_mx_bn_bwd(const msc_mx_bn_bwd_desc* d, void* stream) {
         return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: dy and dres are different buffers; either may be dout, with its row pitch");
     const BnPlan p = bn_plan(d->rows, d->C);
     if (p.ctiles > 65535) return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_bn_bwd: too many channels");
+    const int64_t len = (int64_t)d->C * es, nb = ((int64_t)d->C + BLOCK - 1) / BLOCK;
+    const Rows dout{d->dout, d->dout_ld * es, len, d->rows}, y{d->y, d->y_ld, nb * BLOCK, d->rows}, ys{d->y_scales, d->s_ld, nb, d->rows};
+    const Rows mask{d->relu == 3 ? d->relu_mask : nullptr, d->mask_ld, (d->C + per - 1) / per, d->rows};
+    const Rows dy{d->dy, d->dy_ld * es, len, d->rows}, dres{d->dres, d->dres_ld * es, len, d->rows};
+    for (const Rows& o : {dy, dres})
+        if ((o.p != d->dout && meet(o, dout)) || meet(o, y) || meet(o, ys) || meet(o, mask))
+            return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: dy or dres shares memory with an operand and is not dout itself");
+    if (meet(dy, dres)) return msc_fail(MSC_ERR_ARG, "msc_mx_bn_bwd: dy and dres share memory");
     BnArgs a;
     a.dout = d->dout; a.y = d->y; a.y_scales = d->y_scales; a.mask = d->relu_mask;
     a.mean = d->mean; a.invstd = d->invstd; a.gamma = d->gamma; a.scale = d->scale; a.shift = d->shift;

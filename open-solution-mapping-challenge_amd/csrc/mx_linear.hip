@@ -585,7 +585,13 @@ extern "C" int msc_mx_linear(const msc_mx_linear_desc* d, void* stream) {
     a.res_ld = d->res_ld; a.out_ld = d->out_ld; a.M = d->M; a.K = d->K; a.N = d->N; a.nb = (int)p.nb; a.relu = d->relu; a.tiles_m = a.tiles_n = 0;
     const LinTile t = lin_tile(p, d->M, d->N);
     rc = lin_tile_check(t, p, a);
-    if (rc) return rc;                                         // nothing has been launched so far
+    if (rc) return rc;
+    const Rows out{d->out, d->out_ld * es, (int64_t)d->N * es, d->M}, res{d->res, d->res_ld * es, (int64_t)d->N * es, d->M}, x{d->x, d->x_ld * es, (int64_t)d->K * es, d->M};
+    const Rows xc{d->x ? nullptr : d->x_codes, d->xc_ld, p.nb * E2M1::BYTES, d->M}, xs{d->x ? nullptr : d->x_scales, d->xs_ld, p.nb, d->M};
+    if (meet(out, x) || meet(out, xc) || meet(out, xs) || meet(out, {d->w, d->w_ld, p.nb * E2M1::BYTES, d->N}) || meet(out, {d->w_scales, d->s_ld, p.nb, d->N}))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_linear: out shares memory with x or w: other channels' blocks still read them");
+    if (d->res != d->out && meet(out, res)) return msc_fail(MSC_ERR_ARG, "msc_mx_linear: out shares memory with res and is not res itself");
+    // (nothing has been launched so far)
     if (p.pack) {
         rc = msc_mx_pack(d->x, d->x_ld, d->dtype, codes, p.xc_ld, scales, p.s_ld, MSC_MX_E2M1, d->M, d->K, stream);
         if (rc) return rc;

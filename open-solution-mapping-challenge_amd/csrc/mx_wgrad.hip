@@ -446,6 +446,10 @@ extern "C" int msc_mx_wgrad(const msc_mx_wgrad_desc* d, void* stream) {
     const int64_t hw = (int64_t)d->Hp * d->Wp, image = (int64_t)d->Hq * d->Wq * (d->q_ld > d->s_ld ? d->q_ld : d->s_ld);
     if (((p.chunk - 1) / hw + 2) * image >= 1ll << 31)
         return msc_fail(MSC_ERR_UNSUPPORTED, "msc_mx_wgrad: the images of %d output pixels span 2 GiB", p.chunk);
+    const int64_t dw_bytes = (int64_t)d->A * d->KH * d->KW * d->B * 4, nb = ((int64_t)d->B + BLOCK - 1) / BLOCK, q_rows = (int64_t)d->N * d->Hq * d->Wq;
+    const Rows dw = one_row(d->dw, dw_bytes);
+    if (meet(dw, {d->p, d->p_ld * es, (int64_t)d->A * es, d->N * hw}) || meet(dw, {d->q, d->q_ld, nb * BLOCK, q_rows}) || meet(dw, {d->q_scales, d->s_ld, nb, q_rows}))
+        return msc_fail(MSC_ERR_ARG, "msc_mx_wgrad: dw shares memory with an operand");
     WgArgs a;
     a.p = (const char*)d->p; a.q = d->q; a.qs = d->q_scales; a.dw = d->dw; a.part = (float*)d->ws;
     a.p_ld = d->p_ld; a.q_ld = d->q_ld; a.s_ld = d->s_ld;

@@ -47,3 +47,33 @@ def test_linear_refuses_before_it_launches():
     refused(run(**dict(far, xc_ld=1 << 24, xs_ld=64)), '2 GiB')
     refused(run(**dict(far, xc_ld=1024, xs_ld=1 << 24)), '2 GiB')
     refused(run(**dict(far, xc_ld=1024, xs_ld=64, w_scales=A16, s_ld=1 << 24)), '2 GiB')
+
+
+M = 1 << 20        # addresses far from each other
+
+
+def test_results_that_share_memory_with_operands_are_refused():
+    lib = _lib.load()
+    pk = lambda x, codes, scales, x_ld=64, c_ld=64, s_ld=2, rows=10: lib.msc_mx_pack(x, x_ld, _lib.BF16, codes, c_ld, scales, s_ld, _lib.MX_E4M3, rows, 64, None)  # noqa: E731
+    un = lambda x, codes, scales: lib.msc_mx_unpack(codes, 64, scales, 2, _lib.MX_E4M3, x, 64, _lib.BF16, 10, 64, None)  # noqa: E731
+    for call in (pk, un):
+        refused(call(M, M, 9 * M), 'shares memory')
+        refused(call(M, M + 9 * 128 + 112, 9 * M), 'shares memory')       # the last row's last bytes
+        refused(call(M, 9 * M, M + 40), 'shares memory')
+    refused(pk(M, M + 32, 9 * M, x_ld=256, c_ld=512), 'shares memory')     # inside the rows' columns
+
+    w = lambda **kw: lib.msc_mx_wgrad(C.byref(wgrad_desc(**dict(dict(p=M, q=4 * M, q_scales=8 * M, dw=12 * M, ws=16 * M), **kw))), None)  # noqa: E731
+    for bad in (dict(dw=M), dict(dw=4 * M + 256), dict(dw=8 * M), dict(dw=M - 4), dict(dw=4 * M - 64 * 9 * 64 * 4 + 4)):
+        refused(w(**bad), 'shares memory')
+
+    far = dict(dout=M, y=4 * M, y_scales=8 * M, dy=12 * M, dres=16 * M, dres_ld=64, ws=20 * M, relu=3, relu_mask=24 * M, mask_ld=8)
+    b = lambda **kw: lib.msc_mx_bn_bwd(C.byref(bn_desc(**dict(far, **kw))), None)  # noqa: E731
+    for bad in (dict(dy=M + 128), dict(dy=M - 2), dict(dres=M + 2), dict(dy=4 * M), dict(dres=8 * M), dict(dres=24 * M), dict(dy=16 * M + 64), dict(dy=M + 64, dout_ld=96, dy_ld=96),
+                dict(dy=M + 4, dout_ld=256, dy_ld=128)):
+        refused(b(**bad), 'memory')
+
+    lin = dict(x=M, w=4 * M, w_scales=8 * M, out=12 * M, res=16 * M, res_ld=48, ws=20 * M)
+    n = lambda **kw: lib.msc_mx_linear(C.byref(linear_desc(**dict(lin, **kw))), None)  # noqa: E731
+    for bad in (dict(out=M + 2), dict(out=M - 2), dict(out=4 * M), dict(out=8 * M), dict(out=16 * M + 96), dict(out=16 * M - 2), dict(out=M + 126, x_ld=112, out_ld=112),
+                dict(x=None, x_codes=24 * M, x_scales=28 * M, xc_ld=32, xs_ld=2, out=24 * M), dict(x=None, x_codes=24 * M, x_scales=28 * M, xc_ld=32, xs_ld=2, out=28 * M)):
+        refused(n(**bad), 'memory' if bad.get('out') != 24 * M else 'x')
