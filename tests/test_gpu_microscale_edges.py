@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import mx_ref
-from test_gpu_microscale import DT, U, check_wgrad, f64, values
+from test_gpu_microscale import DT, HALF, TINY, U, check_wgrad, f64, values
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,44 @@ def test_neighbouring_slices_and_overlapping_ones():
     with pytest.raises(_lib.MscError, match='memory'):
         mx.pack(raw[:640].view(10, 64), out=mx.MxTensor(bytes_[2048:2688].view(10, 64), bytes_[8192:8212].view(10, 2), 64))
     assert not raw.any()
+
+
+# ------------------------------------------------------------------------------------------------ BatchNorm backward of wide tensors with many rows
+@pytest.mark.parametrize('dtype,relu', [('bf16', 'bytes'), ('fp16', 'bytes'), ('fp32', 'bytes'), ('bf16', 'coefficients'), ('fp16', 'none')])
+@pytest.mark.parametrize('rows,c', [(2100, 264), (4000, 1030), (9000, 512), (40000, 256)])
+def test_batchnorm_backward_of_wide_tensors(rows, c, relu, dtype):
+    """three launches with whole and several column tiles and hundreds of row ranges, mask and join, against float64 sums on the device.  At these sizes a thread adds 8 rows at most
+    in fp32 (1024 blocks share the rows; what they leave is added in double), so a sum is off by 8 additions and the rounding of the result, dgamma's by the product and the centring as
+    well, relative to the absolute terms -- and not by one per row"""
+    from mapping_challenge_amd import microscale as mx
+    g = torch.Generator(device='cuda').manual_seed(rows + c)
+    rnd = lambda *s: torch.randn(s, generator=g, device='cuda')  # noqa: E731
+    x = (rnd(rows, c) * torch.exp(0.5 * rnd(c)) + 0.5 * rnd(c)).to(DT[dtype])
+    saved = mx.pack(x)
+    y = mx.unpack(saved, torch.float32).double()
+    mean, invstd = y.mean(0).float(), (1 / torch.sqrt(y.var(0, unbiased=False) + 1e-5)).float()
+    gamma, dout = 1 + 0.2 * rnd(c), (rnd(rows, c) * 1e-2 + 1e-3).to(DT[dtype])
+    kw, mask = {}, torch.ones((rows, c), dtype=torch.bool, device='cuda')
+    if relu == 'bytes':
+        per = 4 if dtype == 'fp32' else 8
+        mask = torch.rand((rows, c), generator=g, device='cuda') > 0.4
+        bits = torch.nn.functional.pad(mask, (0, -c % per)).view(rows, -1, per).int()
+        kw['relu_mask'] = (bits << torch.arange(per, device='cuda')).sum(2).to(torch.uint8)
+    elif relu == 'coefficients':
+        scale, shift = gamma * invstd, 0.3 * rnd(c)
+        kw['scale'], kw['shift'] = scale, shift
+        z, size = y * scale.double() + shift.double(), (y * scale.double()).abs() + shift.double().abs()
+        mask = z > 0
+        dout = torch.where(z.abs() > 2 * U * size, dout, torch.zeros_like(dout))      # no gradient where rounding could decide the mask
+    dy, dgamma, dbeta, dres = mx.batchnorm_backward(dout, saved, gamma, mean, invstd, residual=True, **kw)
+    m, i, ga = mean.double(), invstd.double(), gamma.double() * invstd.double()
+    dh = torch.where(mask, dout.double(), torch.zeros((), dtype=torch.float64, device='cuda'))
+    xhat = (y - m) * i
+    db, dg = dh.sum(0), (dh * xhat).sum(0)
+    tb, tg = 9 * U * dh.abs().sum(0), 11 * U * (dh.abs() * (y.abs() + m.abs())).sum(0) * i
+    assert ((dbeta.double() - db).abs() <= tb).all() and ((dgamma.double() - dg).abs() <= tg).all()
+    size = (y.abs() + m.abs()) * i
+    want = ga * (dh - db / rows - xhat * dg / rows)
+    tol = ga.abs() * (4 * U * (dh.abs() + db.abs() / rows + size * dg.abs() / rows) + tb / rows + size * tg / rows) * (1 + HALF[dtype]) + HALF[dtype] * want.abs() + TINY[dtype]
+    assert ((dy.double() - want).abs() <= tol).all()
+    assert torch.equal(dres.double(), dh)
