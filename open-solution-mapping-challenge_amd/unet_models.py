@@ -520,6 +520,8 @@ class UNetResNet(nn.Module):
 
     # ------------------------------------------------------------------ program construction
     def _program(self, N, H, W, training, device):
+        if training and self.activation_checkpoint not in (None, 'e4m3'):      # (an attribute: it may have been set since)
+            raise ValueError("activation_checkpoint must be None or 'e4m3', got %r" % (self.activation_checkpoint,))
         key = (N, H, W, training, self.compute_dtype) + ((self.activation_checkpoint,) if training and self.activation_checkpoint else ())
         prog = self._programs.get(key)
         if prog is None:

@@ -77,3 +77,12 @@ def test_results_that_share_memory_with_operands_are_refused():
     for bad in (dict(out=M + 2), dict(out=M - 2), dict(out=4 * M), dict(out=8 * M), dict(out=16 * M + 96), dict(out=16 * M - 2), dict(out=M + 126, x_ld=112, out_ld=112),
                 dict(x=None, x_codes=24 * M, x_scales=28 * M, xc_ld=32, xs_ld=2, out=24 * M), dict(x=None, x_codes=24 * M, x_scales=28 * M, xc_ld=32, xs_ld=2, out=28 * M)):
         refused(n(**bad), 'memory' if bad.get('out') != 24 * M else 'x')
+
+
+def test_network_option_set_later_is_checked():
+    """the attribute is read when a training program is built: another word would have run as 'e4m3'"""
+    from mapping_challenge_amd.unet_models import UNetResNet
+    net = UNetResNet(34, 2, num_filters=32, dropout_2d=0.0, is_deconv=True)
+    net.activation_checkpoint = 'e5m2'
+    with pytest.raises(ValueError, match='activation_checkpoint'):
+        net._program(1, 64, 64, True, torch.device('cpu'))
