@@ -342,8 +342,10 @@ template <typename T, int RELU> __global__ __launch_bounds__(256) void bn_apply_
 }
 
 // Few rows: one launch.  A block has 16 channels and every row, kept in registers between the sums and the result: nothing is read twice, nothing is joined across
-// blocks.  One launch against three, us on the device: 300 x 256 with join 6.6 : 11.4; 512 x 2048 8.6 : 12.5; 1024 x 2048 11.9 : 14.8; 2048 x 512 without 9.4 : 11.4, with 13.3 : 12.0;
-// 2048 x 2048 19.4 : 19.9 -- and 5 us less of host time.  A CU's lines bound it: 2048 rows, one line each of dout, y and the results for 32 bytes of it.
+// blocks.  One launch against three, us on the device (bf16, a graph of twelve calls), without a join: 1024 x 512 7.0 : 9.4, 1536 x 512 8.0 : 9.6, 2048 x 512 8.9 : 9.8,
+// 2048 x 1024 9.7 : 12.6, 2048 x 2048 14.1 : 17.3; with one: 512 x 256 6.8 : 9.7, 1024 x 512 8.9 : 10.0, 1536 x 512 10.9 : 10.2, 2048 x 256 11.7 : 10.0, 2048 x 512 12.8 : 10.8, 2048 x 1024
+// 15.4 : 13.6, 1536 x 2048 15.6 : 16.5, 2048 x 2048 18.9 : 18.9.  From some 1500 rows on a join is up to 2 us better off with three, and a call from the host 5 us worse off (no workspace
+// to allocate here, one launch): the limit stays one number.  A CU's lines bound the kernel: 2048 rows, one line each of dout, y and the results for 32 bytes of it.
 constexpr int BN_FEW_THREADS = 512, BN_FEW_COLS = 2, BN_FEW_GROUPS = BN_FEW_THREADS / BN_FEW_COLS, BN_FEW_PER = 8, BN_FEW = BN_FEW_GROUPS * BN_FEW_PER;
 
 template <typename T, int RELU> __global__ __launch_bounds__(BN_FEW_THREADS) void bn_few_rows_kernel(BnArgs a) {

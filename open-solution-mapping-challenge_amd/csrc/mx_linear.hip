@@ -10,11 +10,15 @@
 // channels, x quantised by the tile kernel itself; else packing,
 // then tiles of 256 x 256 (fewer: 128 x 128, 64 x 64).
 //
-// What bounds them.  1 x 4096 -> 4096: 6.1 us on the device for 9 MB, one wave's chain of loads; the call takes 8.5 us of host time.  8192 x 1024 -> 256: 12 us for
-// 21 MB, the chain of a step (read, quantise, LDS, products) on two blocks per CU.  8192 x 4096 -> 4096 with a residual: 17.5 us of packing, then 113-125 us of
-// product (275 GFLOP: 2.2-2.4 PFLOP/s).  Taken apart, its requests alone take 49 us (1 GB from the L2s at the 10-11 TB/s they deliver), reads and products
-// 45, the epilogue some 40: 134 MB of residual and result, moved by all CUs in step, with no registers left to hold a tile back (256 in use).  Requesting the
-// residual ahead of the last step spilled (160-180 us); waiting before the stores instead of behind them, 136.
+// What bounds them.  1 x 4096 -> 4096: 5.7 us on the device for 9 MB, one wave's chain of loads; the call takes 8.5 us of host time.  8192 x 1024 -> 256: 11.8 us for
+// 21 MB, the chain of a step (read, quantise, LDS, products) on two blocks per CU.  8192 x 4096 -> 4096 with a residual: 124 us, 17 of them packing (275 GFLOP:
+// 2.2 PFLOP/s).  Taken apart, the product's requests alone take 49 us (512 tiles of 1.1 MB = 0.57 GB from the L2s, 11.6 TB/s), reads and products 45, the epilogue some
+// 40: 134 MB of residual and result, moved by all CUs in step, with no registers left to hold a tile back (256 in use) -- together 134 for a kernel of 113 to 119,
+// so that the three hardly overlap.  Requesting the residual ahead of the last step spilled (160-180 us); waiting before the stores instead of behind them, 136.
+//
+// Next to the 16-bit 1x1 convolution (msc_conv_igemm at its best configuration, bf16, a graph of twelve calls, us): ahead where weights or products dominate, 1 x 4096 -> 4096 5.7
+// : 15.6, 8192 x 4096 -> 4096 with a residual 124 : 246; behind on a ResNet's own layers, whose x and out travel in 16 bits either way: 131072 x 64 -> 256 36.6 : 24.4,
+// 131072 x 256 -> 64 27.0 : 17.4, 32768 x 512 -> 128 15.2 : 10.5, 8192 x 1024 -> 256 11.6 : 9.2, 2048 x 512 -> 2048 with a residual 13.6 : 11.2.  There it saves memory, not time.
 #include <type_traits>
 
 #include "common.h"
@@ -439,7 +443,10 @@ constexpr int64_t FUSED_LDS = 64 * 1024;
 // x quantised by the tile kernel itself (mx_fused_kernel): for up to 64 rows of a short reduction, for weights of at most two waves' channels, and where 512 blocks of 16 (32) x 256 cover the result and the
 // reduction is short.  Measured against packing first, us on the device: 8192 x 1024 -> 256 12.4 : 17.5; 131072 x 256 -> 64 27.5 : 42.0; 32768 x 512 -> 128 15.7 : 21.9;
 // 2048 x 512 -> 2048 12.7 : 15.3; but 8192 x 1024 -> 1024 31.7 : 26.9, 1024 x 4096 -> 1024 29.5 : 22.4, 8192 x 4096 -> 512 48.4 : 43.2, 131072 x 64 -> 256 58.8 : 38.3
-// and 24 x 1024 -> 4096 8.9 : 8.2, 64 x 1024 -> 1024 8.9 : 10.2, 64 x 256 -> 256 5.2 : 8.6, 64 x 4096 -> 128 40 : 16 (packing, then the kernel for few rows)
+// and 24 x 1024 -> 4096 8.9 : 8.2, 64 x 1024 -> 1024 8.9 : 10.2, 64 x 256 -> 256 5.2 : 8.6, 64 x 4096 -> 128 40 : 16 (packing, then the kernel for few rows).
+// Around the limit of 1024 channels, in a graph of twelve calls: 8192 x K -> 256 11.8 : 15.7 (K = 1024), 15.1 : 18.7 (1536), 18.4 : 21.5 (2048), 33.4 : 33.8 (4096); 2048 x K -> 1024
+// 14.9 : 15.5 (1536), 17.9 : 16.8 (2048); 300 x K -> 512 10.7 : 11.6 (1536), 13.0 : 13.0 (2048); 512 x 2048 -> 2048 16.8 : 13.4; 40 x 1024 -> 256 8.4 : 8.7, 64 x 1536 -> 256
+// 10.6 : 9.7, 24 x 2048 -> 1024 12.9 : 8.7.  The crossing lies between 1000 and 4000 with the number of channels and rows; 1024 is the side on which nothing loses
 constexpr int FUSED_CHANNELS = 128, FUSED_BLOCKS = 512, FUSED_K = 1024;
 constexpr int64_t FUSED_MOST = 1ll << 29;      // rows: 2^23 blocks, whose 2^31 threads are within a launch; the form behind the packing has a grid of the card's size
 

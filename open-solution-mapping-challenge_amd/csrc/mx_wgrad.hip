@@ -8,7 +8,7 @@
 // 16-bit input come from HBM, and the conversion is one instruction for two elements, once per block.  The k-contiguous fragments come out of LDS by
 // transposing reads.  The pixel ranges' partial tiles go to the workspace, tile by tile and coalesced, and a second launch adds them in order.
 //
-// What bounds it.  131072 pixels, 256 x 64: HBM (75 MB, 16.5 + 4 us with the join, 19.2 us a call = 4.0 TB/s).  32x16x16, 256 -> 256, 3x3 (9.7 GFLOP, 6 us of
+// What bounds it.  131072 pixels, 256 x 64: HBM (75 MB, 16.6 + 4 us with the join in the profiler, 19.6 us undisturbed = 3.9 TB/s).  32x16x16, 256 -> 256, 3x3 (9.7 GFLOP, 6 us of
 // matrix instructions): latency -- nine steps a group; of 24 us some 9 are launch, first loads and partial sums, and loads, LDS writes, reads and products
 // of a step take about as long as each other and overlap in part.  Divisions in the loop, the depth of the prefetch and the share of VALU
 // work were tried out of it one by one: within 3 %.
@@ -350,7 +350,10 @@ WgPlan wg_plan(const msc_mx_wgrad_desc* d) {
     // Tiles of 128 read less, but are few and take longer to start.  They are for 2^31 products and more where their blocks can fill the card: without splitting the pixels, or with
     // ranges that stay long.  us with the join, 128 : 64, bf16: 8192 pixels, 256 x 256, 3x3 29.8 : 50.3; 6144 27.8 : 39.3; 2048 22.5 : 17.9; 131072, 256 x 64 20.5 : 21.0;
     // 65536, 256 x 64 17.2 : 15.8; 32768, 256 x 256 21.3 : 22.9; 400, 384 x 384, 3x3 19.3 : 12.5; 4096, 128 x 512 13.6 : 11.1; 2048 pixels: 512 x 2048 22.6 : 18.4, 1024 x 2048
-    // 30.3 : 25.7, 2048 x 2048 (256 blocks) 42.6 : 47.9, 512 x 512, 3x3 (144 blocks) 39.6 : 36.7
+    // 30.3 : 25.7, 2048 x 2048 (256 blocks) 42.6 : 47.9, 512 x 512, 3x3 (144 blocks) 39.6 : 36.7.  In a graph of twelve calls, 1x1, at 2048 / 4096 / 8192 pixels: 64 blocks (1024 x 1024) 21.3 :
+    // 17.1 / 28.4 : 27.7 / 41.6 : 49.0; 96 (1024 x 1536) 26.3 : 23.0 / 38.6 : 37.7 / 63.3 : 67.0; 121 30.0 : 23.5 / 43.9 : 39.4 / 70.0 : 70.4; 144 40.3 : 35.2 / 66.1 : 58.0 / 117 : 105;
+    // 160 40.6 : 35.1 / 66.1 : 58.6 / 117 : 107; 192 40.6 : 35.5 / 65.7 : 59.5 / 116 : 109; 256 40.5 : 44.1 / 65.5 : 74.9 / 116 : 135.  What the rule gives away: up to 15 % at 160 to
+    // some 230 blocks, which fill the card's 256 CUs in part, and up to 10 % near 4096 pixels
     const int64_t large = (int64_t)((d->A + 127) / 128) * ((d->B + 127) / 128) * taps;
     const bool wide = M * taps * d->A >= ((1ll << 31) + d->B - 1) / d->B && (large >= 160 || (large <= 128 && M >= 4096));
     p.ta = wide && d->A > 64 ? 128 : 64;

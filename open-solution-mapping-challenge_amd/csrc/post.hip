@@ -913,15 +913,12 @@ struct CrfHaloR {
 // NORM: the normalisers (sum of the kernel weights over the window clipped to the image) instead of one iteration
 template <int R> struct CrfCols { float gx[2 * R + 1], bx[2 * R + 1]; };      // column factors, computed on the host: kernel arguments = SGPR operands
 
-// ---- The same kernel written on PAIRS of pixels.  It was made for packed fp32 instructions (v_pk_*_f32), which the build now switches off (Makefile: wrong
-// results now and then on this hardware); the pairs are compiled to single operations: the tail with CRF and watershed went from 0.037 to 0.042 ms per image.
-// What follows describes the packed form.  ---- round 5: the same kernel on PACKED fp32 math.  The vector peak the roofline quotes (157 TFLOP/s) is the rate of v_pk_fma_f32 -- two
-// lanes' worth of fp32 FMA per issue slot; scalar-fp32 code tops out at half of it, and the round-4 form (13 VALU + 1 v_exp_f32 per tap and
-// pixel, all unpacked) sat at 0.20 of that peak = 0.40 of what unpacked code can reach.  Here a lane's four vertical pixels are two PAIRS
-// (k, k+1): colour differences, squared distance, exponent argument, the Gaussian factor and the four accumulations are v_pk_* over the
-// pair (13 packed ops + 2 v_exp_f32 per tap and pair: ~10.5 issue slots per tap and pixel instead of 17); a pair's window is 12 halo rows
-// (the row that only one of the two pixels reaches runs with a zero / -1e30 factor for the other).  Same arithmetic per element as the
-// unpacked form (IEEE fma either way), so the results agree with it to the last bit wherever the compiler contracts the same products.
+// ---- The same kernel on PAIRS of vertical pixels (k, k + 1): colour differences as floats, squared distance, exponent argument, the Gaussian factor and the four
+// accumulations are written once for a pair, whose window is 12 halo rows (the row that only one of the two pixels reaches runs with a zero / -1e30 factor for the
+// other).  Same arithmetic per element as the unpaired form (IEEE fma either way), so the results agree with it to the last bit wherever the compiler contracts the same
+// products.  The pairs were made for the packed fp32 instructions, which the build switches off (Makefile); compiled to single ones they still beat the unpaired form, whose
+// colour differences are integers: 0.697 against 0.827 ms per 32 images of 256 x 256.  crf_x_kernel below, which runs by default, takes 0.640 (0.49-0.54 while its pairs
+// were packed instructions); MSC_CRF_X=0 and MSC_CRF_PK=0 choose the older ones.
 typedef float crf_f2 __attribute__((ext_vector_type(2)));
 
 template <int R, bool NORM, bool PK = false>
@@ -1087,14 +1084,14 @@ __global__ __launch_bounds__(256, 4) void crf_r_kernel(const float* __restrict__
     }
 }
 
-// ---- round 6: the bilateral kernel on EXACT integer colour distances from a dot product, the Gaussian kernel as a separable blur in its own launch.
+// ---- The bilateral kernel on EXACT integer colour distances from a dot product, the Gaussian kernel as a separable blur in its own launch.
 // (a) The colours are 8-bit: |o - m|^2 = |o|^2 + |m|^2 - 2 o.m, and every term is an integer below 2^24, i.e. exact in fp32 whatever the order -- the
 //     three subtractions and three multiply-adds per tap and pair become one add and three multiply-adds against the centre pixel's -2 m (per halo pixel
 //     |o|^2 is computed once when the tile is loaded; 1e30 outside the image, which zeroes the weight), and the exponent argument is the same
 //     fma(dist, -k, bx + by) as before: the weights are those of crf_r_kernel bit for bit.
 // (b) exp(-(dx^2+dy^2)/2s^2) does not depend on the image: the Gaussian message is a separable 11 + 11 tap blur of Q * n_g (crf_gauss_kernel, ~1/10 of the
-//     multiply-adds of the 121-tap form), its normaliser the product of two 1-D window sums.  The hot loop keeps 8 packed operations + 2 v_exp_f32 per tap
-//     and pixel pair (13 + 2 before), 16 bytes of LDS per halo pixel (20 before).
+//     multiply-adds of the 121-tap form), its normaliser the product of two 1-D window sums.  The hot loop keeps 8 pair operations + 2 v_exp_f32 per tap
+//     and pixel pair (13 + 2 before; a pair operation is two instructions), 16 bytes of LDS per halo pixel (20 before).
 template <int R>
 struct CrfHaloX {
     static constexpr int HW_ = CRF_T + 2 * R;
